@@ -30,6 +30,7 @@ CALIB_LIB_PATH = PKG_DIR / "calib" / "libslm_calib.so"
 QUANT_HEADER_PATH = PKG_DIR.parent / "include" / "slm_quant.h"
 LAYER_HEADER_PATH = PKG_DIR.parent / "include" / "slm_layer.h"
 GGUF_HEADER_PATH = PKG_DIR.parent / "include" / "slm_gguf.h"
+PAGED_HEADER_PATH = PKG_DIR.parent / "include" / "slm_paged.h"
 
 SLM_OK = 0
 ERRORS = {
@@ -192,6 +193,14 @@ SIGNATURES = {
     "slm_model_destroy": (None, [_P]),
     "slm_model_weights_view": (_P, [_P]),
     "slm_model_vocab_size": (ctypes.c_int32, [_P]),
+    # slm_paged.h
+    "slm_paged_create": (ctypes.c_int, [_P, _P, ctypes.POINTER(_P)]),
+    "slm_paged_destroy": (None, [_P]),
+    "slm_paged_device_ptr": (_P, [_P]),
+    "slm_paged_offset": (ctypes.c_size_t, [_P, _I, _I, _I, _I, _I]),
+    "slm_paged_append_dev": (ctypes.c_int, [_P, _P, _I, _P, _P, _P, _P, _P, _P, ctypes.c_float,
+                                            _P]),
+    "slm_paged_attend_dev": (ctypes.c_int, [_P, _P, _I, _P, _P, _I, _I, _P]),
 }
 
 
@@ -228,6 +237,20 @@ class ModelWeightsC(ctypes.Structure):
     """slm_model_weights (include/slm_layer.h)."""
     _fields_ = [("token_embd", _P), ("layers", ctypes.POINTER(LayerWeightsC)),
                 ("num_layers", ctypes.c_int32), ("output_norm", _P), ("lm_head", _P)]
+
+
+class PagedConfigC(ctypes.Structure):
+    """slm_paged_config (include/slm_paged.h)."""
+    _fields_ = [("num_layers", ctypes.c_int32), ("num_pages", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("max_seqs", ctypes.c_int32)]
+
+
+class PagedBatchC(ctypes.Structure):
+    """slm_paged_batch (include/slm_paged.h)."""
+    _fields_ = [("n_seqs", ctypes.c_int32), ("n_rows", ctypes.c_int32),
+                ("max_len", ctypes.c_int32), ("table_stride", ctypes.c_int32),
+                ("page_table", _P), ("lens", _P), ("row_start", _P)]
 
 _lib = None
 
@@ -303,12 +326,15 @@ class AttentionContext:
             raise SlmAttnError(rc, self.lib.slm_attn_last_error(None).decode())
         self._h = h
         self._graphs = weakref.WeakSet()  # live recordings, closed before the context
+        self._caches = weakref.WeakSet()  # live paged caches, the same
 
     # -- lifetime -------------------------------------------------------------
     def close(self) -> None:
         if getattr(self, "_h", None):
             for g in list(getattr(self, "_graphs", ())):
                 g.close()
+            for p in list(getattr(self, "_caches", ())):
+                p.close()
             self.lib.slm_attn_destroy(self._h)
             self._h = None
 
@@ -426,6 +452,18 @@ class AttentionContext:
         c = weights.c()
         self._check(self.lib.slm_layer_forward_dev(self._h, layer, start, n, ctypes.byref(c),
                                                    rms_eps, x))
+
+    # -- paged cache (slm_paged.h) -------------------------------------------------
+    def paged_append_dev(self, cache: "PagedCache", layer: int, batch: "PagedBatch", q, k, v,
+                         q_out, q_norm=0, k_norm=0, norm_eps: float = 1e-5) -> None:
+        self._check(self.lib.slm_paged_append_dev(self._h, cache.handle, layer, batch.ref, q or
+                                                  None, k, v, q_norm or None, k_norm or None,
+                                                  norm_eps, q_out or None))
+
+    def paged_attend_dev(self, cache: "PagedCache", layer: int, batch: "PagedBatch", q_rot, out,
+                         window: int = 0, sinks: int = 0) -> None:
+        self._check(self.lib.slm_paged_attend_dev(self._h, cache.handle, layer, batch.ref, q_rot,
+                                                  window, sinks, out))
 
     # -- the whole model (TransformerModel) ---------------------------------------
     def model_forward_token_dev(self, weights: "ModelWeights", rms_eps: float, token: int,
@@ -576,6 +614,76 @@ class AttentionGraph:
             self.close()
         except Exception:
             pass
+
+
+PAGED_DTYPES = {"f32": 0, "bf16": 1}
+
+
+class PagedCache:
+    """A paged KV cache of a context's heads (slm_paged_create): the pool
+    [layer][page][K|V][kv head][row of page][head_dim] in dtype ("f32" or
+    "bf16").  It keeps its context alive; AttentionContext.close closes it."""
+
+    def __init__(self, ctx: "AttentionContext", num_layers: int, num_pages: int,
+                 page_size: int = 16, dtype: str = "f32", max_seqs: int = 256):
+        self.lib = ctx.lib
+        if dtype not in PAGED_DTYPES:
+            raise ValueError(f"dtype must be one of {sorted(PAGED_DTYPES)}")
+        c = PagedConfigC(num_layers, num_pages, page_size, PAGED_DTYPES[dtype], max_seqs)
+        h = _P()
+        ctx._check(self.lib.slm_paged_create(ctx.handle, ctypes.byref(c), ctypes.byref(h)))
+        self._h = h
+        self._ctx = ctx
+        self.num_layers, self.num_pages, self.page_size = num_layers, num_pages, page_size
+        self.dtype, self.max_seqs = dtype, max_seqs
+        ctx._caches.add(self)
+
+    @property
+    def handle(self):
+        return self._h
+
+    def device_ptr(self) -> int:
+        return self.lib.slm_paged_device_ptr(self._h) or 0
+
+    def offset(self, layer: int, page: int, which: int, kv_head: int, row: int) -> int:
+        """Values from device_ptr() to a row, or -1 (as size_t) out of range."""
+        return int(self.lib.slm_paged_offset(self._h, layer, page, which, kv_head, row))
+
+    def close(self) -> None:
+        """Frees the pool; waits for the context's stream first."""
+        if getattr(self, "_h", None):
+            if self._ctx.handle:
+                rc = self.lib.slm_attn_sync(self._ctx.handle)
+                if rc != SLM_OK:
+                    raise SlmAttnError(rc, "cache not destroyed: " + self.lib.slm_attn_last_error(
+                        self._ctx.handle).decode())
+            self.lib.slm_paged_destroy(self._h)
+            self._h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class PagedBatch:
+    """slm_paged_batch (include/slm_paged.h): device addresses of the int32
+    arrays, whose memory is the caller's to keep alive, and the host's numbers.
+    row_start 0: one row per sequence.  A batch may be used for any number of
+    calls; its fields may be changed in between."""
+
+    def __init__(self, n_seqs: int, page_table: int, table_stride: int, lens: int, max_len: int,
+                 row_start: int = 0, n_rows: int | None = None):
+        self.c = PagedBatchC(n_seqs, n_seqs if n_rows is None else n_rows, max_len, table_stride,
+                             page_table or None, lens or None, row_start or None)
+        self.ref = ctypes.pointer(self.c)
 
 
 class Q4Matrix:
@@ -796,7 +904,8 @@ def header_functions(*headers: os.PathLike | str) -> list[str]:
     """Names of the functions the given headers (default: every include/*.h) declare."""
     import re
 
-    paths = headers or (HEADER_PATH, QUANT_HEADER_PATH, LAYER_HEADER_PATH, GGUF_HEADER_PATH)
+    paths = headers or (HEADER_PATH, QUANT_HEADER_PATH, LAYER_HEADER_PATH, GGUF_HEADER_PATH,
+                        PAGED_HEADER_PATH)
     names = set()
     for h in paths:
         names |= set(re.findall(r"\b(slm_[a-z0-9_]+)\s*\(", Path(h).read_text()))

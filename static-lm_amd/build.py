@@ -24,7 +24,7 @@ BUILD_DIR = PKG_DIR / "_build"
 
 HIP_SOURCES = ["slm_attn.hip", "slm_layer.hip", "slm_model.hip", "rope_append.hip",
                "attn_decode.hip", "prefill_mfma.hip", "prefill_split.hip", "quant_gemm.hip",
-               "norm_act.hip"]
+               "norm_act.hip", "slm_paged.hip", "paged_append.hip", "paged_decode.hip"]
 # measurement probes of the bench, a library of their own (not the product's)
 CALIB_DIR = PKG_DIR / "calib"
 CALIB_LIB = CALIB_DIR / "libslm_calib.so"

@@ -61,6 +61,7 @@ __device__ __forceinline__ float group_sum(float x) {
     if constexpr (LPG >= 8) x += dpp<0x141>(x);   // row_half_mirror
     if constexpr (LPG >= 16) x += dpp<0x140>(x);  // row_mirror
     if constexpr (LPG >= 32) x += __shfl_xor(x, 16);
+    if constexpr (LPG >= 64) x += __shfl_xor(x, 32);
     return x;
 }
 

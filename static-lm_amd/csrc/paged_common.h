@@ -1,0 +1,24 @@
+// What the kernels of the paged cache share (gfx950).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "attn_common.h"
+#include "paged_index.h"
+
+namespace slm {
+
+// paged_row for a row that is the wave's (every lane of it is active): up to 63
+// sequences take one load of the starts and a ballot.
+__device__ __forceinline__ PagedRow paged_row_wave(const PagedView& b, int row) {
+    if (!b.row_start || b.n_seqs >= 64) return paged_row(b, row);
+    const int lane = threadIdx.x & 63;
+    const int start = b.row_start[min(lane, b.n_seqs)];
+    const int below = __popcll(__ballot(lane <= b.n_seqs && start <= row));
+    if (below == 0 || below > b.n_seqs) return PagedRow{-1, -1, false};
+    const int end = min(__builtin_amdgcn_readlane(start, below), b.n_rows);
+    if (row >= end) return PagedRow{-1, -1, false};  // starts that do not ascend
+    return paged_row_of(b, below - 1, end, row);
+}
+
+}  // namespace slm

@@ -1,0 +1,493 @@
+// Attention of single rows over a paged cache: each row's keys are cut into
+// chunks, a workgroup attends one chunk with the query heads of one KV head,
+// and a second kernel joins the chunks.
+//
+//   out_h = sum_t softmax_t(q_h . K[t, g] / sqrt(hd)) V[t, g]   over the rows
+//   t that the row sees, g = h / kv_mul
+//
+// What bounds it: the K and V rows, read once each for up to four query heads
+// of the KV head.  The softmax is one pass (running max m and sum l, log2
+// domain), so nothing else of that size moves.
+//
+// Chunks.  A batch's sequences differ in length, and the host does not know
+// the lengths (they lie on the device, so that a captured graph follows them).
+// Every wave therefore forms the same plan from them: with T_r the tiles of
+// row r's visible keys (one at least), T their sum and U the workgroups per KV
+// head group that fill the card, a chunk is C = ceil(T / U) tiles and row r has
+// ceil(T_r / C) chunks.  That is at most U + n_rows chunks whatever the lengths
+// are, which is the grid; workgroups behind the last chunk end at once.  A row
+// of one chunk is written to out directly.
+//
+// Lanes.  LPG lanes hold one key's head_dim values in 16-byte loads, so a wave
+// attends 64 / LPG keys at a time, each lane group with its own (m, l, o); the
+// states are merged through LDS at the end.  Keys are numbered without the
+// window's gap (Visible), and each lane group looks its page up a tile ahead.
+#include <float.h>
+#include <math.h>
+
+#include "paged_common.h"
+#include "slm_internal.h"
+
+namespace slm {
+namespace {
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes of the cache as floats
+template <class T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void get(u4 x, float (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(x[i]);
+    }
+};
+template <>
+struct Vec<__bf16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void get(u4 x, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(x[i] << 16);
+            f[2 * i + 1] = __uint_as_float(x[i] & 0xFFFF0000u);
+        }
+    }
+};
+
+// Lanes per key (LPG) and keys per lane group and tile (TP).
+template <class T, int HD>
+struct Cfg;
+template <> struct Cfg<float, 16> { static constexpr int LPG = 2, TP = 2; };
+template <> struct Cfg<float, 32> { static constexpr int LPG = 4, TP = 2; };
+template <> struct Cfg<float, 48> { static constexpr int LPG = 4, TP = 2; };
+template <> struct Cfg<float, 64> { static constexpr int LPG = 8, TP = 2; };
+template <> struct Cfg<float, 96> { static constexpr int LPG = 8, TP = 2; };
+template <> struct Cfg<float, 128> { static constexpr int LPG = 16, TP = 2; };
+template <> struct Cfg<float, 256> { static constexpr int LPG = 32, TP = 2; };
+template <> struct Cfg<__bf16, 16> { static constexpr int LPG = 2, TP = 2; };
+template <> struct Cfg<__bf16, 32> { static constexpr int LPG = 4, TP = 2; };
+template <> struct Cfg<__bf16, 48> { static constexpr int LPG = 2, TP = 1; };
+template <> struct Cfg<__bf16, 64> { static constexpr int LPG = 8, TP = 4; };
+template <> struct Cfg<__bf16, 96> { static constexpr int LPG = 4, TP = 1; };
+template <> struct Cfg<__bf16, 128> { static constexpr int LPG = 16, TP = 4; };
+template <> struct Cfg<__bf16, 256> { static constexpr int LPG = 32, TP = 4; };
+
+constexpr int kWaves = 4;
+constexpr int kMaxGb = 4;  // query heads of a workgroup, at most
+
+template <class T, int HD>
+constexpr int tile_rows() {
+    return kWaves * (64 / Cfg<T, HD>::LPG) * Cfg<T, HD>::TP;
+}
+
+struct DecodeParams {
+    PagedView b;
+    const float* q;   // [n_rows][dim], rotated
+    float* out;       // [n_rows][dim]
+    float* part_o;    // [chunk][num_heads][head_dim]
+    float* part_ml;   // [chunk][num_heads][2]
+    int units;        // U, chunks to aim for; 0: every row is one chunk
+    int num_heads;
+    int kv_mul;
+    int gb;           // query heads of a workgroup
+    int window;
+    int sinks;
+    float scale_log2;
+};
+
+__device__ __forceinline__ long long wave_sum_ll(long long x) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+// Where chunk `want` (or the first chunk of row `row_want`) lies.
+struct Chunk {
+    int row;     // -1: behind the last chunk
+    int index;   // within its row
+    int count;   // of its row
+    int tiles;   // C
+    int first;   // the row's first chunk
+};
+
+template <int TILE>
+__device__ __forceinline__ int row_tiles(const DecodeParams& p, int row) {
+    const PagedRow r = paged_row(p.b, row);
+    return max(1, (Visible(r.pos, p.window, p.sinks).count + TILE - 1) / TILE);
+}
+
+// Every lane of the wave gets the same answer.
+template <int TILE>
+__device__ Chunk find_chunk(const DecodeParams& p, int want, int row_want) {
+    const int lane = threadIdx.x & 63;
+    const int n = p.b.n_rows;
+    int mine = lane < n ? row_tiles<TILE>(p, lane) : 0;
+    long long total = mine;
+    for (int r = lane + 64; r < n; r += 64) total += row_tiles<TILE>(p, r);
+    total = wave_sum_ll(total);
+    const int c = (int)((total + p.units - 1) / p.units);
+    int before = 0;  // chunks of the rows in front of this stretch of 64
+    for (int r0 = 0; r0 < n; r0 += 64) {
+        if (r0) mine = r0 + lane < n ? row_tiles<TILE>(p, r0 + lane) : 0;
+        const int cnt = (mine + c - 1) / c;
+        int upto = cnt;  // chunks up to this lane's row
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(upto, o);
+            if (lane >= o) upto += y;
+        }
+        const bool here = row_want >= 0 ? r0 + lane == row_want
+                                        : lane + r0 < n && want < before + upto;
+        const unsigned long long m = __ballot(here);
+        if (m) {
+            const int l = __ffsll(m) - 1;
+            const int k = __shfl(cnt, l), first = before + __shfl(upto, l) - k;
+            return Chunk{r0 + l, want - first, k, c, first};
+        }
+        before += __shfl(upto, 63);
+    }
+    return Chunk{-1, 0, 0, c, 0};
+}
+
+// One online-softmax step over TP keys of a lane group (the first `TP` of the
+// raw registers): the state is rescaled only when some lane's max has grown by
+// more than kLazyRescale.
+template <class T, int HD, int LPG, int NV, int GB, int TP, int TPR>
+__device__ __forceinline__ void attend(const float (&q)[GB][NV][Vec<T>::N], const u4 (&kr)[TPR][NV],
+                                       const u4 (&vr)[TPR][NV], int at, float (&m)[GB],
+                                       float (&l)[GB], float (&o)[GB][NV][Vec<T>::N]) {
+    constexpr int N = Vec<T>::N;
+    float sc[GB][TP];
+#pragma unroll
+    for (int t = 0; t < TP; ++t) {
+#pragma unroll
+        for (int i = 0; i < GB; ++i) sc[i][t] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float f[N];
+            Vec<T>::get(kr[at + t][v], f);
+#pragma unroll
+            for (int i = 0; i < GB; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) sc[i][t] = fmaf(q[i][v][e], f[e], sc[i][t]);
+        }
+    }
+    float pr[GB][TP];
+#pragma unroll
+    for (int i = 0; i < GB; ++i) {
+#pragma unroll
+        for (int t = 0; t < TP; ++t) sc[i][t] = group_sum<LPG>(sc[i][t]);
+        float mx = sc[i][0];
+#pragma unroll
+        for (int t = 1; t < TP; ++t) mx = fmaxf(mx, sc[i][t]);
+        if (__any(mx > m[i] + kLazyRescale)) {  // uniform
+            const float mn = fmaxf(m[i], mx);
+            const float alpha = fast_exp2(m[i] - mn);
+            l[i] *= alpha;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[i][v][e] *= alpha;
+            m[i] = mn;
+        }
+#pragma unroll
+        for (int t = 0; t < TP; ++t) {
+            pr[i][t] = fast_exp2(sc[i][t] - m[i]);
+            l[i] += pr[i][t];
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < TP; ++t)
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float f[N];
+            Vec<T>::get(vr[at + t][v], f);
+#pragma unroll
+            for (int i = 0; i < GB; ++i)
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[i][v][e] = fmaf(pr[i][t], f[e], o[i][v][e]);
+        }
+}
+
+template <class T, int HD, int GB>
+__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(DecodeParams p) {
+    constexpr int LPG = Cfg<T, HD>::LPG, TP = Cfg<T, HD>::TP, N = Vec<T>::N;
+    constexpr int NV = HD / LPG / N;
+    constexpr int GPW = 64 / LPG;
+    constexpr int TILE = tile_rows<T, HD>();
+    constexpr int NS = kWaves * GPW;  // lane-group states of the workgroup
+    static_assert(HD % (LPG * N) == 0, "whole 16-byte loads");
+    const PagedView& b = p.b;
+
+    const int nhb = (p.kv_mul + GB - 1) / GB;
+    const int groups = b.kv_heads * nhb;
+    const int idx = blockIdx.x / groups;
+    const int gy = blockIdx.x - idx * groups;
+    const int g = gy / nhb;
+    const int hb = (gy - g * nhb) * GB;  // this workgroup's heads in the KV head's kv_mul
+    const int h0 = g * p.kv_mul + hb;
+
+    Chunk ch{idx, 0, 1, 0, 0};
+    if (p.units) {
+        ch = find_chunk<TILE>(p, idx, -1);
+        if (ch.row < 0) return;
+    }
+    const PagedRow r = paged_row(b, ch.row);
+    if (r.seq < 0) return;
+    const Visible vis(r.pos, p.window, p.sinks);
+    const int u_beg = ch.index * ch.tiles * TILE;
+    const int u_end = ch.count == 1 ? vis.count : min(vis.count, u_beg + ch.tiles * TILE);
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane % LPG;
+    const int lg = lane / LPG;
+    const T* pages = static_cast<const T*>(b.pages);
+    const int32_t* table = b.table + (size_t)r.seq * b.stride;
+    const int slot_mask = (1 << b.ps_shift) - 1;
+
+    float q[GB][NV][N], m[GB], l[GB], o[GB][NV][N];
+#pragma unroll
+    for (int i = 0; i < GB; ++i) {
+        // a head group's last workgroup may have fewer heads: it computes one twice
+        const float* src = p.q + ((size_t)ch.row * p.num_heads + g * p.kv_mul +
+                                  min(hb + i, p.kv_mul - 1)) * HD;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                const float4 x = ld4(src + N * (v * LPG + li) + e);
+                q[i][v][e] = x.x * p.scale_log2;
+                q[i][v][e + 1] = x.y * p.scale_log2;
+                q[i][v][e + 2] = x.z * p.scale_log2;
+                q[i][v][e + 3] = x.w * p.scale_log2;
+#pragma unroll
+                for (int f = 0; f < 4; ++f) o[i][v][e + f] = 0.0f;
+            }
+        m[i] = -FLT_MAX;  // finite, so that m - m and score - m need no guard
+        l[i] = 0.0f;
+    }
+
+    bool bad_page = false;
+    int page[TP];
+    const auto key = [&](int tb, int tp) {  // the lane group's key of a tile, clamped to the last
+        return vis.row(min(tb + (tp * kWaves + wave) * GPW + lg, u_end - 1));
+    };
+    const auto look_up = [&](int tb) {
+#pragma unroll
+        for (int tp = 0; tp < TP; ++tp) page[tp] = table[key(tb, tp) >> b.ps_shift];
+    };
+    if (u_beg < u_end) look_up(u_beg);
+    for (int tb = u_beg; tb < u_end; tb += TILE) {
+        u4 kr[TP][NV], vr[TP][NV];
+#pragma unroll
+        for (int tp = 0; tp < TP; ++tp) {
+            const bool ok = paged_page_ok(b, page[tp]);
+            bad_page |= !ok;
+            const T* at = pages + paged_at(b, ok ? page[tp] : 0, 0, g, key(tb, tp) & slot_mask, HD);
+            const size_t to_v = ((size_t)b.kv_heads << b.ps_shift) * HD;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const T* a = at + N * (v * LPG + li);
+                kr[tp][v] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a));
+                vr[tp][v] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a + to_v));
+            }
+        }
+        if (tb + TILE < u_end) look_up(tb + TILE);
+        if (tb + TILE <= u_end) {
+            attend<T, HD, LPG, NV, GB, TP, TP>(q, kr, vr, 0, m, l, o);
+        } else {
+            // the last keys: lane groups behind the end sit out, so that what
+            // they loaded is never multiplied
+#pragma unroll
+            for (int tp = 0; tp < TP; ++tp)
+                if (tb + (tp * kWaves + wave) * GPW + lg < u_end)
+                    attend<T, HD, LPG, NV, GB, 1, TP>(q, kr, vr, tp, m, l, o);
+        }
+    }
+
+    // Merge: every lane group scales its state to the workgroup's max into a
+    // slot of its own, each thread sums the slots of one (head, dim).  As many
+    // heads at a time as fit 40 KiB, so that the slots do not limit the
+    // workgroups of a CU.
+    constexpr int HR = NS * GB * HD * 4 <= 40 * 1024 ? GB : 1;
+    __shared__ float s_m[kWaves][GB];
+    __shared__ __align__(16) float s_o[NS][HR][HD];
+    __shared__ float s_l[GB][NS];
+    const float nan = __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < GB; ++i) {
+        const float x = groups_max<LPG>(m[i]);
+        if (lane == 0) s_m[wave][i] = x;
+    }
+    __syncthreads();
+    const int slot = wave * GPW + lg;
+#pragma unroll
+    for (int i0 = 0; i0 < GB; i0 += HR) {
+        if (i0) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < HR; ++j) {
+            const int i = i0 + j;
+            float mw = s_m[0][i];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) mw = fmaxf(mw, s_m[w][i]);
+            const float e = fast_exp2(m[i] - mw);
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int k = 0; k < N; k += 4)
+                    *reinterpret_cast<float4*>(&s_o[slot][j][N * (v * LPG + li) + k]) =
+                        make_float4(o[i][v][k] * e, o[i][v][k + 1] * e, o[i][v][k + 2] * e,
+                                    o[i][v][k + 3] * e);
+            if (li == 0) s_l[i][slot] = bad_page ? nan : l[i] * e;
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < HR * HD; x += 64 * kWaves) {
+            const int j = x / HD, d = x - j * HD, i = i0 + j;
+            if (hb + i >= p.kv_mul) break;
+            float so = 0.0f, sl = 0.0f;
+            for (int s = 0; s < NS; ++s) {
+                so += s_o[s][j][d];
+                sl += s_l[i][s];
+            }
+            const int h = h0 + i;
+            if (ch.count == 1) {
+                // an empty row gives zeros, one of a bad length NaN
+                p.out[((size_t)ch.row * p.num_heads + h) * HD + d] =
+                    r.bad ? nan : vis.count ? so / sl : 0.0f;
+            } else {
+                const size_t at = (size_t)idx * p.num_heads + h;
+                p.part_o[at * HD + d] = so;
+                if (d == 0) {
+                    float mw = s_m[0][i];
+#pragma unroll
+                    for (int w = 1; w < kWaves; ++w) mw = fmaxf(mw, s_m[w][i]);
+                    p.part_ml[2 * at] = mw;
+                    p.part_ml[2 * at + 1] = sl;
+                }
+            }
+        }
+    }
+}
+
+// Joins a row's chunks for one head: a workgroup per (row, head), R rows of
+// threads over the chunks.
+template <class T, int HD>
+__global__ __launch_bounds__(256) void paged_join_kernel(DecodeParams p) {
+    constexpr int TILE = tile_rows<T, HD>();
+    constexpr int R = 256 / HD;  // chunks side by side
+    __shared__ float s_o[R][HD], s_l[R], s_m[4];
+    const int row = blockIdx.x / p.num_heads;
+    const int h = blockIdx.x - row * p.num_heads;
+    const Chunk ch = find_chunk<TILE>(p, 0, row);
+    if (ch.count == 1) return;  // written by its workgroup
+    const int t = threadIdx.x;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+    float mx = -FLT_MAX;
+    for (int c = t; c < ch.count; c += 256)
+        mx = fmaxf(mx, ml[(size_t)(ch.first + c) * p.num_heads + h].x);
+    mx = wave_max(mx);
+    if ((t & 63) == 0) s_m[t >> 6] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    const int k = t / HD, d = t - k * HD;
+    if (k < R) {
+        float so = 0.0f, sl = 0.0f;
+        for (int c = k; c < ch.count; c += R) {
+            const size_t at = (size_t)(ch.first + c) * p.num_heads + h;
+            const float2 x = ml[at];
+            const float e = fast_exp2(x.x - mx);
+            sl += e * x.y;
+            so += e * p.part_o[at * HD + d];
+        }
+        s_o[k][d] = so;
+        if (d == 0) s_l[k] = sl;
+    }
+    __syncthreads();
+    if (t < HD) {
+        float so = s_o[0][t], sl = s_l[0];
+#pragma unroll
+        for (int i = 1; i < R; ++i) {
+            so += s_o[i][t];
+            sl += s_l[i];
+        }
+        p.out[((size_t)row * p.num_heads + h) * HD + t] = so / sl;
+    }
+}
+
+// Workgroups per KV head group that fill the card with two waves per SIMD.
+int units_of(const Shape& s, int groups) {
+    const int wgs = 2 * s.cus;
+    return groups >= wgs ? 1 : wgs / groups;
+}
+
+// Query heads of a workgroup: kv_mul in equal parts of at most four.
+int gb_of(int kv_mul) {
+    const int parts = (kv_mul + kMaxGb - 1) / kMaxGb;
+    return (kv_mul + parts - 1) / parts;
+}
+
+int groups_of(const Shape& s) {
+    const int gb = gb_of(s.kv_mul);
+    return s.num_kv_heads * ((s.kv_mul + gb - 1) / gb);
+}
+
+template <class T, int HD>
+hipError_t launch_t(const Shape& s, DecodeParams p, hipStream_t st) {
+    const int groups = groups_of(s);
+    // no sequence has more tiles than this
+    const int most = (p.b.max_len + tile_rows<T, HD>() - 1) / tile_rows<T, HD>();
+    if (p.units && (long)most * p.b.n_rows < p.units) p.units = most * p.b.n_rows;
+    if (most == 1) p.units = 0;
+    const long wgs = ((long)p.units + p.b.n_rows) * groups;
+    if (wgs > (1L << 30) / 256 || (long)p.b.n_rows * s.num_heads > (1L << 30) / 256)
+        return hipErrorInvalidValue;
+    const dim3 grid((unsigned)wgs);
+    switch (p.gb) {
+        case 1: hipLaunchKernelGGL((paged_decode_kernel<T, HD, 1>), grid, dim3(256), 0, st, p); break;
+        case 2: hipLaunchKernelGGL((paged_decode_kernel<T, HD, 2>), grid, dim3(256), 0, st, p); break;
+        case 3: hipLaunchKernelGGL((paged_decode_kernel<T, HD, 3>), grid, dim3(256), 0, st, p); break;
+        default: hipLaunchKernelGGL((paged_decode_kernel<T, HD, 4>), grid, dim3(256), 0, st, p);
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !p.units) return e;
+    hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(p.b.n_rows * s.num_heads), dim3(256), 0,
+                       st, p);
+    return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_hd(const Shape& s, const DecodeParams& p, hipStream_t st) {
+    switch (s.head_dim) {
+        case 16: return launch_t<T, 16>(s, p, st);
+        case 32: return launch_t<T, 32>(s, p, st);
+        case 48: return launch_t<T, 48>(s, p, st);
+        case 64: return launch_t<T, 64>(s, p, st);
+        case 96: return launch_t<T, 96>(s, p, st);
+        case 128: return launch_t<T, 128>(s, p, st);
+        case 256: return launch_t<T, 256>(s, p, st);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+size_t paged_decode_chunks(const Shape& s, int max_rows) {
+    return (size_t)units_of(s, groups_of(s)) + max_rows;
+}
+
+hipError_t launch_paged_decode(const Shape& s, const PagedView& b, bool bf16, const float* q,
+                               int window, int sinks, float* part_o, float* part_ml, float* out,
+                               hipStream_t st) {
+    const int gb = gb_of(s.kv_mul);
+    const DecodeParams p{b,      q,     out,
+                         part_o, part_ml, part_o ? units_of(s, groups_of(s)) : 0,
+                         s.num_heads, s.kv_mul, gb,
+                         window, sinks, 1.4426950408889634f / sqrtf((float)s.head_dim)};
+    return bf16 ? launch_hd<__bf16>(s, p, st) : launch_hd<float>(s, p, st);
+}
+
+}  // namespace slm

@@ -198,4 +198,19 @@ hipError_t launch_q4_gemv_q8_argmax(const Q4Job& job, const uint32_t* aq, const 
 hipError_t launch_argmax_parts(const ArgmaxPart* parts, int n_parts, const float* x, int32_t* out,
                                hipStream_t st);
 
+// The paged cache (paged_*.hip, slm_paged.h) of one layer.
+struct PagedView;
+// bf16: the pages' type (f32 otherwise); q and the norms may be nullptr
+hipError_t launch_paged_append(const Shape& s, const PagedView& b, bool bf16, const float* q,
+                               const float* k, const float* v, const float* q_norm,
+                               const float* k_norm, float eps, const float* cos_t,
+                               const float* sin_t, float* q_out, hipStream_t st);
+// One row at a time, its keys split into chunks whose partial results go to
+// part_o [chunks][num_heads][head_dim] and part_ml [chunks][num_heads][2], of
+// paged_decode_chunks(rows) chunks; without them nothing is split.
+size_t paged_decode_chunks(const Shape& s, int max_rows);
+hipError_t launch_paged_decode(const Shape& s, const PagedView& b, bool bf16, const float* q,
+                               int window, int sinks, float* part_o, float* part_ml, float* out,
+                               hipStream_t st);
+
 }  // namespace slm
