@@ -24,7 +24,8 @@ BUILD_DIR = PKG_DIR / "_build"
 
 HIP_SOURCES = ["slm_attn.hip", "slm_layer.hip", "slm_model.hip", "rope_append.hip",
                "attn_decode.hip", "prefill_mfma.hip", "prefill_split.hip", "quant_gemm.hip",
-               "norm_act.hip", "slm_paged.hip", "paged_append.hip", "paged_decode.hip"]
+               "norm_act.hip", "slm_paged.hip", "paged_append.hip", "paged_decode.hip",
+               "paged_prefill.hip"]
 # measurement probes of the bench, a library of their own (not the product's)
 CALIB_DIR = PKG_DIR / "calib"
 CALIB_LIB = CALIB_DIR / "libslm_calib.so"
@@ -49,9 +50,10 @@ HIP_FLAGS = [
 ]
 # per-source extras: MFMA results of the Q4_0 GEMM and the split-bf16 prefill go
 # straight to VGPRs (their VALU work reads every one; accumulator registers
-# would cost a v_accvgpr_read per element)
+# would cost a v_accvgpr_read per element); so do the paged prefill's
 HIP_SOURCE_FLAGS = {"quant_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-                    "prefill_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+                    "prefill_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                    "paged_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _run(cmd: list[str]) -> None:

@@ -84,8 +84,8 @@ int check_call(slm_attn_ctx* c, const slm_paged_cache* cache, int layer,
         return fail(c, SLM_ERR_BATCH,
                     "max_len must be positive and at most max_seq_len and the table's rows");
     // workgroups of 256 threads are counted in 24 bits
-    if (!b->row_start && (int64_t)b->n_rows * s.num_heads >= INT64_C(1) << 23)
-        return fail(c, SLM_ERR_BATCH, "n_seqs * num_heads must be below 2^23");
+    if ((int64_t)b->n_rows * s.num_heads + (int64_t)b->n_seqs * s.num_kv_heads >= INT64_C(1) << 23)
+        return fail(c, SLM_ERR_BATCH, "too many rows and heads in one call (2^23)");
     return SLM_OK;
 }
 
@@ -249,11 +249,16 @@ int slm_paged_attend_dev(slm_attn_ctx* c, slm_paged_cache* cache, int32_t layer,
     const slm::PagedView view = view_of(cache, layer, b);
     const OnDevice on(c->device);
     const bool bf16 = cache->cfg.dtype == SLM_PAGED_BF16;
-    const bool split = !b->row_start;
+    if (b->row_start) {
+        Timed t(c, SLM_K_PREFILL);
+        const hipError_t e =
+            slm::launch_paged_prefill(s, view, bf16, q_rot, window, sinks, out, c->stream);
+        t.done();
+        return launch_status(c, e, "paged prefill kernel launch");
+    }
     Timed t(c, SLM_K_DECODE);
     const hipError_t e = slm::launch_paged_decode(s, view, bf16, q_rot, window, sinks,
-                                                  split ? cache->part_o : nullptr, cache->part_ml,
-                                                  out, c->stream);
+                                                  cache->part_o, cache->part_ml, out, c->stream);
     t.done();
     return launch_status(c, e, "paged decode kernel launch");
 }
