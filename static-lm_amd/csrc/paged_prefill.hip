@@ -29,6 +29,7 @@
 // times the f32 MFMA rate, or one f32 product), the softmax between them next.
 #include <float.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include "paged_common.h"
 #include "slm_internal.h"
@@ -51,6 +52,9 @@ struct PrefillParams {
     PagedView b;
     const float* q;
     float* out;
+    float* part_o;   // [item][kv head][BM][head_dim]
+    float* part_ml;  // [item][kv head][BM][2]
+    int units;       // items to aim for; 0: no tile is split
     int num_heads;
     int kv_mul;
     int window;
@@ -71,6 +75,29 @@ constexpr int v_stride(bool bf, int ch) {
     if (!bf) return ch + (ch % 4 == 2 ? 0 : 2);
     while (ch % 16 != 4 && ch % 16 != 12) ch += 2;
     return ch;
+}
+
+// Bytes of one buffer of K and V tiles in LDS, and what a CU has for them.
+template <class T, int HD, int KSP>
+constexpr int tile_bytes() {
+    constexpr int CH = HD * (int)sizeof(T) / 16;
+    return KSP * KT * 16 * (k_stride(CH) + v_stride(sizeof(T) == 2, CH));
+}
+constexpr int kLds = 160 * 1024 - 256;
+
+// Two buffers, unless only one fits.
+template <class T, int HD, int KSP>
+constexpr int buffers() {
+    return 2 * tile_bytes<T, HD, KSP>() <= kLds ? 2 : 1;
+}
+
+// Waves of a SIMD that the registers are held to: two, unless the tiles in LDS,
+// or q and the output alone (hd 256), leave room for one only.
+template <class T, int HD, int RG, int KSP>
+constexpr int waves_per_simd() {
+    if (HD > 128) return 1;
+    if (RG * KSP == 8) return 2;
+    return 2 * buffers<T, HD, KSP>() * tile_bytes<T, HD, KSP>() <= kLds ? 2 : 1;
 }
 
 // Two values as bf16 pairs: x = p1 + p2 + p3 (24 bits).
@@ -120,73 +147,230 @@ __device__ __forceinline__ bool not_finite(u4 x) {
     return any != 0;
 }
 
-// A tile of packed rows of one sequence.
+// A tile of packed rows of one sequence, and a chunk of its steps.
 struct Tile {
-    int seq;    // -1: none
-    int index;  // within the sequence
-    int row0;   // the sequence's first row of the batch
-    int rows;   // and how many it has
+    int seq;     // -1: none
+    int index;   // within the sequence
+    int row0;    // the sequence's first row of the batch
+    int rows;    // and how many it has
+    int len;     // as the batch has it
+    int chunk;   // within the tile
+    int steps;   // of a chunk, at most
+    int item0;   // the tile's first chunk, counted over the batch; chunk c is item0 - c
 };
 
-// Tile `want` of the batch, the last one first (a sequence's last rows see the
-// most keys).  Every lane of the wave gets the same answer.
-template <int BM>
-__device__ Tile find_tile(const PrefillParams& p, int want) {
+constexpr int kUnsplit = 1 << 29;  // steps of a chunk that is the whole tile
+
+// Item (chunk of a tile) `want` of the batch, or with by_tile the first one of
+// tile `want`; the last ones first (a sequence's last rows see the most keys).
+// With p.units, chunks are so long that about that many make up the batch: a
+// sequence of n tiles, none of more than T steps, has n * ceil(T / C) items, C =
+// ceil(sum of n * T over the sequences / units).  Every lane of the wave gets
+// the same answer.
+template <int BM, int KS>
+__device__ Tile find_tile(const PrefillParams& p, int want, bool by_tile) {
     const PagedView& b = p.b;
-    const int lane = threadIdx.x & 63;
-    const auto rows_of = [&](int s, int* first) {
+    struct Seq {
+        int first, rows, len, tiles, steps;
+    };
+    const auto seq_of = [&](int s) {
         const int lo = paged_min(paged_max(b.row_start[s], 0), b.n_rows);
-        *first = lo;
-        return paged_min(paged_max(b.row_start[s + 1], lo), b.n_rows) - lo;
+        const int rows = paged_min(paged_max(b.row_start[s + 1], lo), b.n_rows) - lo;
+        const int len = b.lens[s];
+        long long keys = len < 0 || len > b.max_len ? 0 : len;
+        if (p.window > 0) keys = min(keys, (long long)p.window + p.sinks + BM / p.kv_mul + 2);
+        return Seq{lo, rows, len, (int)(((long long)rows * p.kv_mul + BM - 1) / BM),
+                   max(1, (int)((keys + KS - 1) / KS))};
     };
-    const auto tiles_of = [&](int rows) {
-        return (int)(((long long)rows * p.kv_mul + BM - 1) / BM);
+    const auto chunk_steps = [&](long long total) {
+        return p.units ? max(1, (int)((total + p.units - 1) / p.units)) : kUnsplit;
     };
-    int before = 0;
-    for (int top = b.n_seqs; top > 0; top -= 64) {
-        const int s = top - 1 - lane;  // lane 0 has the last sequence
-        int first = 0, rows = 0, cnt = 0;
-        if (s >= 0) {
-            rows = rows_of(s, &first);
-            cnt = tiles_of(rows);
+    if (b.n_seqs == 1) {  // nothing to look for
+        const Seq q = seq_of(0);
+        const int c = chunk_steps((long long)q.tiles * q.steps);
+        const int k = (q.steps + c - 1) / c, items = q.tiles * k;
+        const int at = (by_tile ? q.tiles : items) - 1 - want;
+        const int index = by_tile ? at : at / k;
+        return Tile{at < 0 ? -1 : 0, index, q.first, q.rows, q.len, by_tile ? 0 : at - index * k, c,
+                    items - 1 - index * k};
+    }
+    // stretches of 64 sequences, the last one first; lane 0 has the last sequence
+    const int lane = threadIdx.x & 63;
+    const auto mine = [&](int top) {
+        const int s = top - 1 - lane;
+        return s >= 0 ? seq_of(s) : Seq{0, 0, 0, 0, 1};
+    };
+    const Seq q0 = mine(b.n_seqs);
+    int c = kUnsplit;
+    if (p.units) {
+        long long total = (long long)q0.tiles * q0.steps;
+        for (int top = b.n_seqs - 64; top > 0; top -= 64) {
+            const Seq q = mine(top);
+            total += (long long)q.tiles * q.steps;
         }
-        int upto = cnt;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
+        c = chunk_steps(total);
+    }
+    const auto upto = [&](int x) {  // sum over the lanes up to this one
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(upto, o);
-            if (lane >= o) upto += y;
+            const int y = __shfl_up(x, o);
+            if (lane >= o) x += y;
         }
-        const unsigned long long m = __ballot(want < before + upto);
+        return x;
+    };
+    int before = 0, items_before = 0;
+    for (int top = b.n_seqs; top > 0; top -= 64) {
+        const Seq q = top == b.n_seqs ? q0 : mine(top);
+        const int k = (q.steps + c - 1) / c;
+        const int items = upto(q.tiles * k);
+        const int cnt = by_tile ? upto(q.tiles) : items;
+        const unsigned long long m = __ballot(want < before + cnt);
         if (m) {
             const int l = __ffsll(m) - 1;
-            const int end = before + __builtin_amdgcn_readlane(upto, l);
+            const int at = before + __builtin_amdgcn_readlane(cnt, l) - 1 - want;
+            const int kl = __builtin_amdgcn_readlane(k, l);
+            const int end = items_before + __builtin_amdgcn_readlane(items, l);
+            const int index = __builtin_amdgcn_readfirstlane(by_tile ? at : at / kl);
             return Tile{__builtin_amdgcn_readfirstlane(top - 1 - l),
-                        __builtin_amdgcn_readfirstlane(end - 1 - want),
-                        __builtin_amdgcn_readlane(first, l), __builtin_amdgcn_readlane(rows, l)};
+                        index,
+                        __builtin_amdgcn_readlane(q.first, l),
+                        __builtin_amdgcn_readlane(q.rows, l),
+                        __builtin_amdgcn_readlane(q.len, l),
+                        __builtin_amdgcn_readfirstlane(by_tile ? 0 : at - index * kl),
+                        __builtin_amdgcn_readfirstlane(c),
+                        __builtin_amdgcn_readfirstlane(end - 1 - index * kl)};
         }
-        before += __builtin_amdgcn_readlane(upto, 63);
+        before += __builtin_amdgcn_readlane(cnt, 63);
+        items_before += __builtin_amdgcn_readlane(items, 63);
     }
-    return Tile{-1, 0, 0, 0};
+    return Tile{-1, 0, 0, 0, 0, 0, 0, 0};
 }
 
-template <class T, int HD, int KSP>
-__global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_kernel(
-    PrefillParams p) {
+// Where a tile lies, and the keys that any of its rows sees: Visible of the
+// last row, from the first row's window on.
+template <int BM, int KS>
+struct Span {
+    int packed;  // packed rows of the sequence
+    int x0;      // the tile's first
+    int pos0;    // position of the sequence's first row; of a bad length all are negative
+    int pos_first, pos_last;  // of the tile's rows
+    bool bad;
+    Visible vis;
+    int steps;   // of KS keys
+    int chunks;
+    __device__ __forceinline__ Span(const PrefillParams& p, const Tile& t) : vis(-1, 0, 0) {
+        const int len = t.len;
+        bad = len < 0 || len > p.b.max_len;
+        packed = t.rows * p.kv_mul;
+        x0 = t.index * BM;
+        pos0 = bad ? -t.rows : len - t.rows;
+        pos_first = max(0, pos0 + x0 / p.kv_mul);
+        pos_last = pos0 + (min(x0 + BM, packed) - 1) / p.kv_mul;
+        vis = Visible(pos_last, 0, 0);
+        if (pos_last >= 0 && p.window > 0) {
+            vis.lo = max(0, pos_first + 1 - p.window);
+            vis.first = min(p.sinks, vis.lo);
+            vis.count = vis.first + pos_last + 1 - vis.lo;
+        }
+        steps = (vis.count + KS - 1) / KS;
+        chunks = max(1, (steps + t.steps - 1) / t.steps);
+    }
+};
+
+// Packed rows x, x + step, .. < end of a tile again, one after another by a wave
+// that goes through the keys u_beg .. u_end - 1 of vis 64 at a time: scores with
+// a key per lane, then the sum with dims over the lanes, in which a key that the
+// row does not see has no part.  For the rare tile whose V the matrix cores
+// cannot take.  The state goes to m, l and o of the row: into out, or the
+// partials of row `part` + x.
+template <class T, int HD>
+__device__ __noinline__ void attend_again(const PrefillParams& p, const Tile& tile, int g,
+                                          const Visible& vis, int u_beg, int u_end, int x, int end,
+                                          int step, int pos0, bool bad, bool whole, size_t part) {
+    constexpr int NL = (HD + 63) / 64;  // dims of a lane
+    const PagedView& b = p.b;
+    const int lane = threadIdx.x & 63;
+    const T* pages = static_cast<const T*>(b.pages);
+    const int32_t* table = b.table + (size_t)tile.seq * b.stride;
+    const int slot_mask = (1 << b.ps_shift) - 1;
+    for (; x < end; x += step) {
+        const int j = x / p.kv_mul;
+        const int pos = pos0 + j, pos_out = p.window > 0 ? pos - p.window : -1;
+        const size_t at = ((size_t)(tile.row0 + j) * p.num_heads + g * p.kv_mul + x -
+                           j * p.kv_mul) * HD;
+        float m = -FLT_MAX, l = 0.0f, o[NL] = {};
+        for (int u0 = u_beg; u0 < u_end; u0 += 64) {
+            const int n = min(64, u_end - u0);
+            const int t = vis.row(min(u0 + lane, u_end - 1));
+            const bool sees = lane < n && t <= pos && !(t <= pos_out && t >= p.sinks);
+            const int page = table[t >> b.ps_shift];
+            const bool ok = paged_page_ok(b, page);
+            const T* k = pages + paged_at(b, ok ? page : 0, 0, g, t & slot_mask, HD);
+            float s = 0.0f;
+            for (int d = 0; d < HD; ++d) s = fmaf(p.q[at + d], (float)k[d], s);
+            s = !ok ? __builtin_nanf("") : s * p.scale_log2;
+            const float mn = fmaxf(m, wave_max(sees ? s : -INFINITY));
+            const float alpha = fast_exp2(m - mn);
+            const float e = sees ? fast_exp2(s - mn) : 0.0f;
+            m = mn;
+            l = l * alpha + wave_sum(e);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) o[i] *= alpha;
+            const unsigned long long who = __ballot(sees);
+            for (int c = 0; c < n; ++c) {
+                if (!(who >> c & 1)) continue;
+                const float ec = __shfl(e, c);
+                const int tc = vis.row(u0 + c);
+                const int pc = table[tc >> b.ps_shift];
+                const T* v = pages + paged_at(b, paged_page_ok(b, pc) ? pc : 0, 1, g,
+                                              tc & slot_mask, HD);
+#pragma unroll
+                for (int i = 0; i < NL; ++i) {
+                    const int d = min(64 * i + lane, HD - 1);
+                    o[i] = fmaf(ec, (float)v[d], o[i]);
+                }
+            }
+        }
+        if (!whole && lane == 0) {
+            p.part_ml[2 * (part + x)] = m;
+            p.part_ml[2 * (part + x) + 1] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            if (64 * i + lane < HD) {
+                if (whole)
+                    p.out[at + 64 * i + lane] =
+                        bad ? __builtin_nanf("") : pos < 0 ? 0.0f : o[i] / l;
+                else
+                    p.part_o[(part + x) * HD + 64 * i + lane] = o[i];
+            }
+    }
+}
+
+template <class T, int HD, int RG, int KSP>
+__global__ __launch_bounds__(64 * RG * KSP, (waves_per_simd<T, HD, RG, KSP>())) void
+paged_prefill_kernel(PrefillParams p) {
     constexpr bool BF = sizeof(T) == 2;
-    constexpr int RG = 4 / KSP;            // groups of packed rows
+    constexpr int NW = RG * KSP, NT = 64 * NW;
     constexpr int BM = 32 * RG;            // packed rows of a workgroup
     constexpr int KS = KSP * KT;           // keys of a step
     constexpr int CV = 16 / sizeof(T);     // values of a chunk
     constexpr int CH = HD / CV;            // chunks of a row
-    constexpr int NC = (KS * CH + kThreads - 1) / kThreads;  // a thread's chunks of K (and V)
-    constexpr bool EXACT = KS * CH % kThreads == 0;
+    constexpr int NC = (KS * CH + NT - 1) / NT;  // a thread's chunks of K (and V)
+    constexpr bool EXACT = KS * CH % NT == 0;
     constexpr int NQ = HD / 16;            // 16-dim steps of K . Q^T
     constexpr int ND = (HD + 31) / 32;     // 32-dim tiles of O^T
     constexpr bool DPAD = HD % 32 != 0;    // the last of them is half empty
     constexpr int KST = k_stride(CH), VST = v_stride(BF, CH);
-    __shared__ u4 s_k[2][KS * KST], s_v[2][KS * VST];
-    __shared__ float s_p[4][16][32];  // merge of the key splits; see `mixed` below
-    __shared__ float s_ml[KSP > 1 ? 4 : 1][2][32];
+    constexpr int MT = KSP == 2 ? (ND + 1) / 2 : ND;  // tiles of O^T that a wave gives away
+    // K tiles, then V tiles, NB buffers each; at the end the key splits' states
+    constexpr int NB = buffers<T, HD, KSP>();
+    constexpr int KW = NB * KS * KST, VW = NB * KS * VST, MERGE = KSP > 1 ? NW * (MT * 256 + 16) : 0;
+    __shared__ u4 s_tiles[KW + VW > MERGE ? KW + VW : MERGE];
+    u4* const s_k = s_tiles;
+    u4* const s_v = s_tiles + KW;
 
     const PagedView& b = p.b;
     const int tid = threadIdx.x;
@@ -196,37 +380,29 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
     const int rg = wave / KSP, ksp = wave % KSP;
 
     const int g = blockIdx.x % b.kv_heads;
-    const Tile tile = find_tile<BM>(p, blockIdx.x / b.kv_heads);
+    const int item = blockIdx.x / b.kv_heads;
+    const Tile tile = find_tile<BM, KS>(p, item, false);
     if (tile.seq < 0) return;  // uniform
-    const int len = b.lens[tile.seq];
-    const bool bad = len < 0 || len > b.max_len;
-    const int packed = tile.rows * p.kv_mul;
-    const int x0 = tile.index * BM;  // first packed row
-    const int pos0 = bad ? -tile.rows : len - tile.rows;  // position of the sequence's first row
+    const Span<BM, KS> span(p, tile);
+    if (tile.chunk >= span.chunks) return;
+    const int st_beg = tile.chunk * tile.steps;
+    const int st_end = min(span.steps, st_beg + tile.steps);
+    const Visible& vis = span.vis;
+    const bool bad = span.bad;
+    const int packed = span.packed, x0 = span.x0, pos0 = span.pos0;
+    const int pos_first = span.pos_first;
     const int x = x0 + rg * 32 + n;  // this lane's packed row
     const bool row_ok = x < packed;
     const int j = min(x, packed - 1) / p.kv_mul;
     const int head = g * p.kv_mul + min(x, packed - 1) - j * p.kv_mul;
     const int pos = pos0 + j;  // < 0: an empty row
     const int pos_out = p.window > 0 ? pos - p.window : -1;  // the last row behind the window
-    // positions of the workgroup's first and last row
-    const int pos_first = max(0, pos0 + x0 / p.kv_mul);
-    const int pos_last = pos0 + (min(x0 + BM, packed) - 1) / p.kv_mul;
-    // and of the wave's
+    // positions of the wave's rows
     const int xw = x0 + rg * 32;
     const bool wave_ok = xw < packed;
     const int wpos_first = max(0, pos0 + xw / p.kv_mul);
     const int wpos_last = pos0 + (min(xw + 32, packed) - 1) / p.kv_mul;
 
-    // the keys that any of the rows sees: Visible(pos_last), from the first
-    // row's window on
-    Visible vis(pos_last, 0, 0);
-    if (pos_last >= 0 && p.window > 0) {
-        vis.lo = max(0, pos_first + 1 - p.window);
-        vis.first = min(p.sinks, vis.lo);
-        vis.count = vis.first + pos_last + 1 - vis.lo;
-    }
-    const int steps = (vis.count + KS - 1) / KS;
     const T* pages = static_cast<const T*>(b.pages);
     const int32_t* table = b.table + (size_t)tile.seq * b.stride;
     const int slot_mask = (1 << b.ps_shift) - 1;
@@ -236,7 +412,7 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
     int page[NC];
     u4 kr[NC], vr[NC];
     unsigned lost = 0;  // bit 2i: chunk i's page is bad; bit 2i + 1: it lies behind the end
-    const auto key_of = [&](int st, int i) { return st * KS + (tid + i * kThreads) / CH; };
+    const auto key_of = [&](int st, int i) { return st * KS + (tid + i * NT) / CH; };
     const auto look_up = [&](int st) {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
@@ -252,16 +428,16 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
             if (u >= vis.count) lost |= 2u << (2 * i);
             const int t = vis.row(min(u, vis.count - 1));
             const T* at = pages + paged_at(b, ok ? page[i] : 0, 0, g, t & slot_mask, HD) +
-                          (tid + i * kThreads) % CH * CV;
+                          (tid + i * NT) % CH * CV;
             kr[i] = *reinterpret_cast<const u4*>(at);
             vr[i] = *reinterpret_cast<const u4*>(at + to_v);
         }
     };
     // Into LDS.  Rows behind the end are zeros; of a bad page K is NaN, so that
     // the scores of the rows that see it are.  Whether V holds a value that is
-    // not finite is asked for where some rows do not see it.
+    // not finite is asked for where some rows do not see it (ask).
+    bool odd = false;
     const auto stage = [&](int buf, bool ask) {
-        bool odd = false;
         if (__any(lost != 0)) {
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
@@ -274,13 +450,12 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
         }
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int e = tid + i * kThreads, row = e / CH;
+            const int e = tid + i * NT, row = e / CH;
             if (!EXACT && row >= KS) break;
-            s_k[buf][row * KST + e % CH] = kr[i];
-            s_v[buf][row * VST + e % CH] = vr[i];
+            s_k[buf * KS * KST + row * KST + e % CH] = kr[i];
+            s_v[buf * KS * VST + row * VST + e % CH] = vr[i];
             if (ask) odd |= not_finite<T>(vr[i]);
         }
-        return odd;
     };
 
     // ---- q ----
@@ -290,6 +465,9 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
     bf8 qb[BF ? NQ : 1][3];
     float qf[BF ? 1 : NQ][8];
     {
+        // the first pages' ids are asked for first, then q, then the first keys
+        const bool any = st_beg < st_end;
+        if (any) look_up(st_beg);
         const float* src = p.q + ((size_t)(tile.row0 + j) * p.num_heads + head) * HD + 8 * half;
         float xq[NQ][8];
 #pragma unroll
@@ -298,6 +476,10 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
             const float v[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) xq[i][e] = v[e];
+        }
+        if (any) {
+            fetch(st_beg);
+            if (st_beg + 1 < st_end) look_up(st_beg + 1);
         }
         if constexpr (BF) {
             float top = 0.0f;
@@ -335,9 +517,9 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
     float m = -FLT_MAX, l = 0.0f;  // finite m: a row that has seen no key yet needs no guard
 
     // ---- one tile of the wave ----
-    const auto attend = [&](int buf, int u0, bool mixed) {
-        const u4* sk = &s_k[buf][ksp * KT * KST];
-        const u4* sv = &s_v[buf][ksp * KT * VST];
+    const auto attend = [&](int buf, int u0) {
+        const u4* sk = s_k + (buf * KS + ksp * KT) * KST;
+        const u4* sv = s_v + (buf * KS + ksp * KT) * VST;
         v16 s = v16{};
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
@@ -364,7 +546,6 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
         const bool gap = u0 < vis.first && u0 + KT > vis.first;
         const bool hidden = gap || t0 + KT - 1 > wpos_first ||
                             (p.window > 0 && u0 >= vis.first && t0 <= wpos_last - p.window);
-        unsigned unseen = 0;
         if (hidden) {  // uniform
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -372,7 +553,6 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
                 const int t = u + (u < vis.first ? 0 : vis.lo - vis.first);
                 const bool hide = (t > pos) | ((t <= pos_out) & (t >= p.sinks));
                 s[r] = hide ? -INFINITY : s[r];
-                unseen |= (unsigned)hide << r;
             }
         }
         float mx = s[0];
@@ -394,35 +574,6 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
             ps += s[r];
         }
         l += ps;
-        if (mixed && hidden) {
-            // V holds an infinity or a NaN, and some rows do not see some keys
-            // (0 * inf is NaN in a product): one key after another, by the
-            // rows that see it.
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    s_p[wave][8 * (r / 4) + 4 * half + r % 4][n] =
-                        unseen >> (8 * ks + r) & 1 ? -1.0f : s[8 * ks + r];
-                __builtin_amdgcn_wave_barrier();
-                for (int k = 0; k < 16; ++k) {
-                    const float pk = s_p[wave][k][n];
-                    if (pk < 0.0f) continue;
-                    const int row = 16 * ks + k;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const int dim = min(32 * d + 8 * (r / 4) + 4 * half + r % 4, HD - 1);
-                            const T* c = reinterpret_cast<const T*>(
-                                &sv[row * VST + dim / CV]);
-                            o[d][r] = fmaf(pk, (float)c[dim % CV], o[d][r]);
-                        }
-                }
-                __builtin_amdgcn_wave_barrier();
-            }
-            return;
-        }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             if constexpr (BF) {
@@ -466,71 +617,96 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
     };
 
     // ---- the steps ----
-    if (steps > 0) {  // uniform
-        look_up(0);
-        fetch(0);
-        if (steps > 1) look_up(1);
-        for (int st = 0; st < steps; ++st) {
-            const int u = st * KS, t = vis.row(u);
+    if (st_beg < st_end) {  // uniform
+        for (int st = st_beg; st < st_end; ++st) {
+            const int u = st * KS, t = vis.row(u), buf = NB == 2 ? st & 1 : 0;
             // some row of the workgroup does not see some key of the step
             const bool ask = u + KS > vis.count || t + KS - 1 > pos_first || p.window > 0;
-            const bool odd = stage(st & 1, ask);
-            if (st + 1 < steps) {
+            stage(buf, ask);
+            if (st + 1 < st_end) {
                 fetch(st + 1);
-                if (st + 2 < steps) look_up(st + 2);
+                if (st + 2 < st_end) look_up(st + 2);
             }
-            bool mixed = false;
-            if (ask)
-                mixed = __syncthreads_or(odd);
-            else
-                __syncthreads();
+            __syncthreads();
             const int u0 = u + ksp * KT;
             // a wave whose rows are all empty or in front of the tile has
             // nothing to do there
-            if (wave_ok && u0 < vis.count && vis.row(u0) <= wpos_last) attend(st & 1, u0, mixed);
+            if (wave_ok && u0 < vis.count && vis.row(u0) <= wpos_last) attend(buf, u0);
+            if (NB == 1) __syncthreads();
         }
     }
     l += other_half(l);
+    // an infinity or a NaN in V where some rows do not see it: 0 * inf is NaN
+    // in a product, so the rows are computed again, key by key
+    const bool redo = __syncthreads_or(odd);  // (and every wave is done with the tiles)
 
-    // ---- key splits, then the output ----
+    // ---- key splits ----
     if constexpr (KSP > 1) {
-        // every wave scales its state to the row's max over the splits, split 0
-        // adds the others' in order
+        // Every wave scales its state to the row's max over the splits.  Split k
+        // sums tiles k, k + KSP, .. of O^T, which the others leave it in the
+        // bytes of the K and V tiles.
+        float* const s_o = reinterpret_cast<float*>(s_tiles);
+        float* const s_ml = s_o + NW * MT * 1024;
+        const auto slot = [&](int w, int d) {
+            return s_o + (w * MT + (KSP == 2 ? d / 2 : d)) * 1024 + lane;
+        };
         if (half == 0) {
-            s_ml[wave][0][n] = m;
-            s_ml[wave][1][n] = l;
+            s_ml[wave * 64 + n] = m;
+            s_ml[wave * 64 + 32 + n] = l;
         }
         __syncthreads();
         float top = m;
 #pragma unroll
-        for (int k = 0; k < KSP; ++k) top = fmaxf(top, s_ml[rg * KSP + k][0][n]);
+        for (int k = 0; k < KSP; ++k) top = fmaxf(top, s_ml[(rg * KSP + k) * 64 + n]);
         const float e = fast_exp2(m - top);
+        m = top;
         l = 0.0f;
 #pragma unroll
         for (int k = 0; k < KSP; ++k)
-            l += s_ml[rg * KSP + k][1][n] * fast_exp2(s_ml[rg * KSP + k][0][n] - top);
+            l += s_ml[(rg * KSP + k) * 64 + 32 + n] *
+                 fast_exp2(s_ml[(rg * KSP + k) * 64 + n] - top);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             o[d] *= e;
-            if (ksp)
+            if (d % KSP != ksp)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s_p[wave][2 * r + half][n] = o[d][r];
-            __syncthreads();
-            if (!ksp)
-#pragma unroll
-                for (int k = 1; k < KSP; ++k)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[d][r] += s_p[wave + k][2 * r + half][n];
-            __syncthreads();
+                for (int r = 0; r < 16; ++r) slot(wave, d)[64 * r] = o[d][r];
         }
-        if (ksp) return;
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            if (d % KSP != ksp) continue;  // uniform
+#pragma unroll
+            for (int k = 1; k < KSP; ++k) {
+                const int w = rg * KSP + (ksp + k) % KSP;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] += slot(w, d)[64 * r];
+            }
+        }
+    }
+
+    // ---- the output ----
+    const bool whole = span.chunks == 1;
+    const size_t part = ((size_t)item * b.kv_heads + g) * BM;  // the tile's first partial row
+    if (redo) {  // uniform
+        if (wave_ok)
+            attend_again<T, HD>(p, tile, g, vis, st_beg * KS, min(vis.count, st_end * KS),
+                                xw + ksp, min(xw + 32, packed), KSP, pos0, bad, whole, part - x0);
+        return;
     }
     if (!row_ok) return;
-    // an empty row gives zeros, one of a bad length NaN
-    const float inv = bad ? __builtin_nanf("") : pos < 0 ? 0.0f : 1.0f / l;
     float* dst = p.out + ((size_t)(tile.row0 + j) * p.num_heads + head) * HD;
+    // an empty row gives zeros, one of a bad length NaN
+    float inv = bad ? __builtin_nanf("") : pos < 0 ? 0.0f : 1.0f / l;
+    if (!whole) {  // uniform
+        const size_t r = part + rg * 32 + n;
+        if (half == 0 && ksp == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * r) = make_float2(m, l);
+        dst = p.part_o + r * HD;
+        inv = 1.0f;
+    }
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
+    for (int d = 0; d < ND; ++d) {
+        if (d % KSP != ksp) continue;
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const int dim = 32 * d + 8 * (r / 4) + 4 * half;
@@ -538,23 +714,122 @@ __global__ __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) void paged_prefill_ker
             *reinterpret_cast<float4*>(dst + dim) = make_float4(o[d][r] * inv, o[d][r + 1] * inv,
                                                                 o[d][r + 2] * inv, o[d][r + 3] * inv);
         }
+    }
 }
 
-template <class T, int HD, int KSP>
-hipError_t launch_k(const Shape& s, const PrefillParams& p, hipStream_t st) {
-    constexpr int BM = 32 * (4 / KSP);
-    // at most this many tiles, whatever the rows' division among the sequences
-    const long tiles = (long)p.b.n_rows * s.kv_mul / BM + p.b.n_seqs;
-    const long wgs = tiles * s.num_kv_heads;
-    if (wgs >= (1L << 32) / kThreads) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((paged_prefill_kernel<T, HD, KSP>), dim3((unsigned)wgs), dim3(kThreads), 0,
-                       st, p);
+// Joins the chunks of a tile for one KV head: four dims of a packed row per
+// thread.
+template <int HD, int BM, int KS>
+__global__ __launch_bounds__(kThreads) void paged_prefill_join_kernel(PrefillParams p) {
+    constexpr int PARTS = (BM * HD / 4 + kThreads - 1) / kThreads;  // workgroups of a tile
+    const PagedView& b = p.b;
+    const int part = blockIdx.x % PARTS, g = blockIdx.x / PARTS % b.kv_heads;
+    const Tile tile = find_tile<BM, KS>(p, blockIdx.x / (PARTS * b.kv_heads), true);
+    if (tile.seq < 0) return;
+    const Span<BM, KS> span(p, tile);
+    if (span.chunks == 1) return;  // written by its workgroup
+    const int e = part * kThreads + threadIdx.x;
+    const int row = e / (HD / 4), dim = e % (HD / 4) * 4;
+    const int x = span.x0 + row;
+    if (row >= BM || x >= span.packed) return;
+    const size_t first = ((size_t)tile.item0 * b.kv_heads + g) * BM + row;
+    const size_t back = (size_t)b.kv_heads * BM;  // from a chunk to the one before
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+    float m = -FLT_MAX, l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    // eight chunks in flight; those behind the last repeat it with weight 0
+    for (int c0 = 0; c0 < span.chunks; c0 += 8) {
+        float2 y[8];
+        float4 z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const size_t r = first - min(c0 + i, span.chunks - 1) * back;
+            y[i] = ml[r];
+            z[i] = ld4(p.part_o + r * HD + dim);
+        }
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mn = fmaxf(mn, y[i].x);
+        const float a = fast_exp2(m - mn);
+        m = mn;
+        l *= a;
+        o.x *= a, o.y *= a, o.z *= a, o.w *= a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (c0 + i >= span.chunks) break;
+            const float w = fast_exp2(y[i].x - m);
+            l += w * y[i].y;
+            o.x = fmaf(w, z[i].x, o.x);
+            o.y = fmaf(w, z[i].y, o.y);
+            o.z = fmaf(w, z[i].z, o.z);
+            o.w = fmaf(w, z[i].w, o.w);
+        }
+    }
+    const int j = x / p.kv_mul;
+    const int head = g * p.kv_mul + x - j * p.kv_mul;
+    const float inv = span.pos0 + j < 0 ? 0.0f : 1.0f / l;  // an empty row gives zeros
+    *reinterpret_cast<float4*>(p.out + ((size_t)(tile.row0 + j) * p.num_heads + head) * HD + dim) =
+        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// At most this many tiles of BM packed rows, whatever the rows' division among
+// the sequences.
+long tiles_bound(const PagedView& b, int kv_mul, int bm) {
+    return ((long)b.n_rows * kv_mul + (long)b.n_seqs * (bm - 1)) / bm;
+}
+
+// No row sees more keys than this.
+long keys_bound(const PrefillParams& p) {
+    const long w = (long)p.window + p.sinks;
+    return p.window > 0 && w < p.b.max_len ? w : p.b.max_len;
+}
+
+template <class T, int HD, int RG, int KSP>
+hipError_t launch_k(const Shape& s, PrefillParams p, hipStream_t st) {
+    constexpr int BM = 32 * RG, KS = KSP * KT, NT = 64 * RG * KSP;
+    static_assert(tile_bytes<T, HD, KSP>() <= kLds, "the tiles fit a CU");
+    const long tiles = tiles_bound(p.b, s.kv_mul, BM);
+    // Tiles that leave CUs empty are split into as many chunks as still run side
+    // by side, if that takes four steps or more off the longest (a second launch
+    // to join them costs about 6 us, a step 1.5 to 3).
+    const long ns = s.cus / (tiles * s.num_kv_heads);
+    const long steps = (keys_bound(p) + KS - 1) / KS;
+    p.units = ns >= 2 && steps * (ns - 1) >= 4 * ns ? (int)(ns * tiles) : 0;
+    const long wgs = (tiles + p.units) * s.num_kv_heads;
+    if (wgs >= (1L << 32) / NT) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((paged_prefill_kernel<T, HD, RG, KSP>), dim3((unsigned)wgs), dim3(NT), 0, st,
+                       p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !p.units) return e;
+    constexpr int parts = (BM * HD / 4 + kThreads - 1) / kThreads;
+    hipLaunchKernelGGL((paged_prefill_join_kernel<HD, BM, KS>),
+                       dim3((unsigned)(tiles * s.num_kv_heads * parts)), dim3(kThreads), 0, st, p);
     return hipGetLastError();
 }
 
+// Groups of packed rows and key splits of a workgroup.
 template <class T, int HD>
 hipError_t launch_t(const Shape& s, const PrefillParams& p, hipStream_t st) {
-    return launch_k<T, HD, 1>(s, p, st);
+    const long wgs = tiles_bound(p.b, s.kv_mul, 128) * s.num_kv_heads;  // with four groups
+    const long keys = keys_bound(p);
+    static const int ek = getenv("SLM_KSP") ? atoi(getenv("SLM_KSP")) : 0;  // TEMP
+    if (ek == 1) return launch_k<T, HD, 4, 1>(s, p, st);
+    if constexpr (HD <= 128) if (ek == 2) return launch_k<T, HD, 4, 2>(s, p, st);
+    if constexpr (HD > 128) {
+        if (wgs <= s.cus / 8) return launch_k<T, HD, 2, 2>(s, p, st);
+    } else if constexpr (HD > 64) {
+        if constexpr (sizeof(T) == 4) {
+            if (keys > 32 && wgs <= s.cus / 4 &&
+                (keys <= 512 || (long)p.b.n_rows * s.kv_mul <= 64L * p.b.n_seqs))
+                return launch_k<T, HD, 1, 4>(s, p, st);
+        }
+        if (keys > 128 && wgs < 3 * s.cus) return launch_k<T, HD, 4, 2>(s, p, st);
+    } else if (keys > 64) {
+        if (wgs <= s.cus * 5 / 16) return launch_k<T, HD, 1, 8>(s, p, st);
+        if (wgs <= s.cus * 5 / 8) return launch_k<T, HD, 2, 4>(s, p, st);
+        if (wgs < 3 * s.cus) return launch_k<T, HD, 4, 2>(s, p, st);
+    }
+    return launch_k<T, HD, 4, 1>(s, p, st);
 }
 
 template <class T>
@@ -573,9 +848,14 @@ hipError_t launch_hd(const Shape& s, const PrefillParams& p, hipStream_t st) {
 
 }  // namespace
 
+// Items times KV heads are at most tiles (fewer than CUs where they are split)
+// and the CUs again; a tile has at most 128 rows.
+size_t paged_prefill_part_rows(const Shape& s) { return (size_t)2 * s.cus * 128; }
+
 hipError_t launch_paged_prefill(const Shape& s, const PagedView& b, bool bf16, const float* q,
-                                int window, int sinks, float* out, hipStream_t st) {
-    const PrefillParams p{b,      q,     out, s.num_heads, s.kv_mul, window,
+                                int window, int sinks, float* part_o, float* part_ml, float* out,
+                                hipStream_t st) {
+    const PrefillParams p{b,      q,     out, part_o, part_ml, 0, s.num_heads, s.kv_mul, window,
                           sinks, 1.4426950408889634f / sqrtf((float)s.head_dim)};
     return bf16 ? launch_hd<__bf16>(s, p, st) : launch_hd<float>(s, p, st);
 }

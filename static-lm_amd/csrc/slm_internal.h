@@ -212,8 +212,11 @@ size_t paged_decode_chunks(const Shape& s, int max_rows);
 hipError_t launch_paged_decode(const Shape& s, const PagedView& b, bool bf16, const float* q,
                                int window, int sinks, float* part_o, float* part_ml, float* out,
                                hipStream_t st);
-// Runs of rows (b.row_start is set), on the matrix cores.
+// Runs of rows (b.row_start is set), on the matrix cores; the parts have room for
+// paged_prefill_part_rows() rows of [head_dim] and [2].
+size_t paged_prefill_part_rows(const Shape& s);
 hipError_t launch_paged_prefill(const Shape& s, const PagedView& b, bool bf16, const float* q,
-                                int window, int sinks, float* out, hipStream_t st);
+                                int window, int sinks, float* part_o, float* part_ml, float* out,
+                                hipStream_t st);
 
 }  // namespace slm

@@ -19,7 +19,7 @@ struct slm_paged_cache {
     int ps_shift = 0;
     void* pool = nullptr;
     size_t layer_bytes = 0;
-    // split-decode partials
+    // partial results of split rows and tiles
     float* part_o = nullptr;
     float* part_ml = nullptr;
 };
@@ -150,14 +150,16 @@ int slm_paged_create(slm_attn_ctx* ctx, const slm_paged_config* cfg, slm_paged_c
         return fail(ctx, SLM_ERR_CONFIG, "the pool would exceed 64 TiB");
     }
     c->layer_bytes = (size_t)cfg->num_pages * 2 * cfg->page_size * s.kv_dim * value_bytes(c);
-    const size_t heads = slm::paged_decode_chunks(s, cfg->max_seqs) * s.num_heads;
+    const size_t chunks = slm::paged_decode_chunks(s, cfg->max_seqs) * s.num_heads;
+    const size_t rows = slm::paged_prefill_part_rows(s);
+    const size_t parts = chunks > rows ? chunks : rows;
     int prev = -1;
     if (hipGetDevice(&prev) != hipSuccess) prev = -1;
     hipError_t e = hipSetDevice(c->device);
     const char* what = "hipMalloc(paged cache)";
     if (e == hipSuccess) e = hipMalloc(&c->pool, pool_bytes(c));
-    if (e == hipSuccess) e = hipMalloc(&c->part_o, heads * s.head_dim * sizeof(float));
-    if (e == hipSuccess) e = hipMalloc(&c->part_ml, heads * 2 * sizeof(float));
+    if (e == hipSuccess) e = hipMalloc(&c->part_o, parts * s.head_dim * sizeof(float));
+    if (e == hipSuccess) e = hipMalloc(&c->part_ml, parts * 2 * sizeof(float));
     if (e == hipSuccess) {
         what = "hipMemset(paged cache)";
         e = hipMemset(c->pool, 0, pool_bytes(c));
@@ -252,7 +254,8 @@ int slm_paged_attend_dev(slm_attn_ctx* c, slm_paged_cache* cache, int32_t layer,
     if (b->row_start) {
         Timed t(c, SLM_K_PREFILL);
         const hipError_t e =
-            slm::launch_paged_prefill(s, view, bf16, q_rot, window, sinks, out, c->stream);
+            slm::launch_paged_prefill(s, view, bf16, q_rot, window, sinks, cache->part_o,
+                                      cache->part_ml, out, c->stream);
         t.done();
         return launch_status(c, e, "paged prefill kernel launch");
     }
