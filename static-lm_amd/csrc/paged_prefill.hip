@@ -5,31 +5,36 @@
 // All of them read the same K and V, so a tile of them is as good as a tile of
 // rows of one head, whatever kv_mul is, and short runs fill a tile sooner.
 //
-// Tiling.  A workgroup has four waves: RG groups of 32 packed rows and KSP key
-// splits (RG * KSP = 4).  A step stages KSP tiles of 32 keys in LDS, row by
-// row and double-buffered: the next step's rows are on their way from their
-// pages into registers while this one is attended, and the pages of the one
-// after that are being looked up.  Keys are numbered without the window's gap
-// (Visible of the workgroup's rows).  Per wave and tile, with 32x32 MFMAs:
+// Tiling.  A workgroup has RG groups of 32 packed rows and KSP key splits, a
+// wave for each.  A step stages KSP tiles of 32 keys in LDS, row by row: the
+// next step's rows are on their way from their pages into registers while this
+// one is attended, and the pages of the one after that are being looked up.
+// Keys are numbered without the window's gap (Visible of the workgroup's rows).
+// Per wave and tile, with v_mfma_f32_32x32x16_bf16:
 //   S^T = K . Q^T    A = K rows, B = Q^T (registers): lane (n = l % 32, h = l /
 //                    32) ends with the scores of packed row n against keys
 //                    8 (r / 4) + 4 h + r % 4 in register r;
 //   O^T = V^T . P^T  B = P^T: a lane supplies its own probabilities, so they
 //                    never move between lanes; A = V^T with its keys in that
-//                    order (bf16: a transposing LDS read; f32: plain reads).
+//                    order, by transposing LDS reads.
+// Few tiles are split over workgroups as well (find_tile), and joined by a
+// second kernel.
 //
-// Precision.  f32 pages: v_mfma_f32_32x32x2_f32.  bf16 pages: K and V are bf16
-// as they are; q and p are split into three bf16 values (24 bits, each the
-// rounded remainder of the ones before), three v_mfma_f32_32x32x16_bf16 for a
-// product, exact up to f32's rounding of the sums.  q is first scaled by a
-// power of two per row, so that no value of any size leaves bf16's exponents;
-// the scores' scale takes it back.
+// Precision.  An f32 value is the sum of three bf16 values (24 bits, each the
+// rounded remainder of the ones before).  bf16 pages: q and p are split so, K
+// and V are what they are: three products, exact but for f32's rounding of the
+// sums.  f32 pages: K and V are split too when they are staged, and of the nine
+// products the three below 2^-25 are left out.  q is first scaled by a power of
+// two per row, so that values of any size stay within bf16's exponents; the
+// scores' scale takes it back.  What cannot be split or must not be multiplied
+// (V from 2^64 on, infinities and NaN among them; with f32 pages also K, and
+// values between 0 and 2^-100, whose remainders run out of exponents) makes the
+// workgroup compute its rows again in plain f32 (attend_again).
 //
-// What bounds it: the matrix cores for long runs (three bf16 products at 16
-// times the f32 MFMA rate, or one f32 product), the softmax between them next.
+// What bounds it: the matrix cores for long runs, the softmax and the splitting
+// between the products next.
 #include <float.h>
 #include <math.h>
-#include <stdlib.h>
 
 #include "paged_common.h"
 #include "slm_internal.h"
@@ -42,6 +47,7 @@ typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float v16 __attribute__((ext_vector_type(16)));
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u2 __attribute__((ext_vector_type(2)));
 
@@ -64,31 +70,36 @@ struct PrefillParams {
 
 // Distance of rows in LDS, in 16-byte chunks (16 of which are all banks).  A K
 // read takes the same chunk of 32 rows: an odd distance gives 16 neighbouring
-// rows all banks.  A V read takes four neighbouring chunks of rows 4 h + (0..3)
-// (bf16, transposing: a distance of 4 or 12 modulo 16 spreads four rows over
-// all banks) or eight of rows 4 h + r (f32: 2 modulo 4 puts the two rows side
-// by side).  As the distances are constants, so are the offsets of a lane's
-// reads; slots chosen by an exclusive or of row bits meet no conflicts either,
-// but need an address register for each read.
+// rows all banks.  A V read takes four neighbouring chunks of rows 4 h + (0..3):
+// a distance of 4 or 12 modulo 16 spreads four rows over all banks.  As the
+// distances are constants, so are the offsets of a lane's reads; slots chosen by
+// an exclusive or of row bits meet no conflicts either, but need an address
+// register for each read.
 constexpr int k_stride(int ch) { return ch | 1; }
-constexpr int v_stride(bool bf, int ch) {
-    if (!bf) return ch + (ch % 4 == 2 ? 0 : 2);
+constexpr int v_stride(int ch) {
     while (ch % 16 != 4 && ch % 16 != 12) ch += 2;
     return ch;
+}
+
+// bf16 planes of a K or V value.
+template <class T>
+constexpr int planes() {
+    return sizeof(T) == 2 ? 1 : 3;
 }
 
 // Bytes of one buffer of K and V tiles in LDS, and what a CU has for them.
 template <class T, int HD, int KSP>
 constexpr int tile_bytes() {
-    constexpr int CH = HD * (int)sizeof(T) / 16;
-    return KSP * KT * 16 * (k_stride(CH) + v_stride(sizeof(T) == 2, CH));
+    return KSP * KT * 16 * planes<T>() * (k_stride(HD / 8) + v_stride(HD / 8));
 }
 constexpr int kLds = 160 * 1024 - 256;
 
-// Two buffers, unless only one fits.
-template <class T, int HD, int KSP>
+// Two buffers, unless only one lets the CU hold eight waves (where the registers
+// do: q and the output of hd 256 leave room for four).
+template <class T, int HD, int RG, int KSP>
 constexpr int buffers() {
-    return 2 * tile_bytes<T, HD, KSP>() <= kLds ? 2 : 1;
+    constexpr int wgs = RG * KSP == 4 && HD <= 128 ? 2 : 1;
+    return 2 * wgs * tile_bytes<T, HD, KSP>() <= kLds ? 2 : 1;
 }
 
 // Waves of a SIMD that the registers are held to: two, unless the tiles in LDS,
@@ -97,7 +108,7 @@ template <class T, int HD, int RG, int KSP>
 constexpr int waves_per_simd() {
     if (HD > 128) return 1;
     if (RG * KSP == 8) return 2;
-    return 2 * buffers<T, HD, KSP>() * tile_bytes<T, HD, KSP>() <= kLds ? 2 : 1;
+    return 2 * tile_bytes<T, HD, KSP>() <= kLds ? 2 : 1;
 }
 
 // Two values as bf16 pairs: x = p1 + p2 + p3 (24 bits).
@@ -134,18 +145,35 @@ __device__ __forceinline__ float other_half(float x) {
     return __uint_as_float((threadIdx.x & 32) ? a[0] : a[1]);
 }
 
+// The largest magnitudes of the values that a thread has staged, and the
+// smallest that are not zero; outside() whether they ask for attend_again.
 template <class T>
-__device__ __forceinline__ bool not_finite(u4 x) {
-    uint32_t any = 0;
+struct Range;
+template <>
+struct Range<__bf16> {
+    us2 top{};  // of the even and the odd values
+    __device__ __forceinline__ void add(u4 x) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 2)
-            any |= ((x[i] & 0x7F807F80u) + 0x00800080u) & 0x80008000u;
-        else
-            any |= ((x[i] & 0x7F800000u) + 0x00800000u) & 0x80000000u;
+        for (int i = 0; i < 4; ++i)
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, x[i] & 0x7FFF7FFFu));
     }
-    return any != 0;
-}
+    __device__ __forceinline__ bool outside() const { return max(top[0], top[1]) >= 0x5F80; }
+};
+template <>
+struct Range<float> {
+    uint32_t top = 0, low = 0xFFFFFFFFu;  // low: bits less one, so that 0 is the largest
+    __device__ __forceinline__ void add(u4 x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = x[i] & 0x7FFFFFFFu;
+            top = max(top, u);
+            low = min(low, u - 1);
+        }
+    }
+    __device__ __forceinline__ bool outside() const {
+        return top >= 0x5F800000u || low < 0x0D800000u - 1;  // 2^64, 2^-100
+    }
+};
 
 // A tile of packed rows of one sequence, and a chunk of its steps.
 struct Tile {
@@ -282,7 +310,7 @@ struct Span {
 // Packed rows x, x + step, .. < end of a tile again, one after another by a wave
 // that goes through the keys u_beg .. u_end - 1 of vis 64 at a time: scores with
 // a key per lane, then the sum with dims over the lanes, in which a key that the
-// row does not see has no part.  For the rare tile whose V the matrix cores
+// row does not see has no part.  For the rare tile whose K or V the matrix cores
 // cannot take.  The state goes to m, l and o of the row: into out, or the
 // partials of row `part` + x.
 template <class T, int HD>
@@ -356,18 +384,21 @@ paged_prefill_kernel(PrefillParams p) {
     constexpr int NW = RG * KSP, NT = 64 * NW;
     constexpr int BM = 32 * RG;            // packed rows of a workgroup
     constexpr int KS = KSP * KT;           // keys of a step
-    constexpr int CV = 16 / sizeof(T);     // values of a chunk
-    constexpr int CH = HD / CV;            // chunks of a row
+    constexpr int CH = HD / 8;             // 16-byte chunks of a row's plane
     constexpr int NC = (KS * CH + NT - 1) / NT;  // a thread's chunks of K (and V)
     constexpr bool EXACT = KS * CH % NT == 0;
+    constexpr int NL = BF ? 1 : 2;         // 16-byte loads of a chunk's values
+    constexpr int NP = planes<T>();
     constexpr int NQ = HD / 16;            // 16-dim steps of K . Q^T
     constexpr int ND = (HD + 31) / 32;     // 32-dim tiles of O^T
     constexpr bool DPAD = HD % 32 != 0;    // the last of them is half empty
-    constexpr int KST = k_stride(CH), VST = v_stride(BF, CH);
+    constexpr int KST = k_stride(CH), VST = v_stride(CH);
     constexpr int MT = KSP == 2 ? (ND + 1) / 2 : ND;  // tiles of O^T that a wave gives away
-    // K tiles, then V tiles, NB buffers each; at the end the key splits' states
-    constexpr int NB = buffers<T, HD, KSP>();
-    constexpr int KW = NB * KS * KST, VW = NB * KS * VST, MERGE = KSP > 1 ? NW * (MT * 256 + 16) : 0;
+    // K tiles, then V tiles, NB buffers of NP planes each; at the end the key
+    // splits' states
+    constexpr int NB = buffers<T, HD, RG, KSP>();
+    constexpr int KW = NB * NP * KS * KST, VW = NB * NP * KS * VST;
+    constexpr int MERGE = KSP > 1 ? NW * (MT * 256 + 16) : 0;
     __shared__ u4 s_tiles[KW + VW > MERGE ? KW + VW : MERGE];
     u4* const s_k = s_tiles;
     u4* const s_v = s_tiles + KW;
@@ -390,7 +421,6 @@ paged_prefill_kernel(PrefillParams p) {
     const Visible& vis = span.vis;
     const bool bad = span.bad;
     const int packed = span.packed, x0 = span.x0, pos0 = span.pos0;
-    const int pos_first = span.pos_first;
     const int x = x0 + rg * 32 + n;  // this lane's packed row
     const bool row_ok = x < packed;
     const int j = min(x, packed - 1) / p.kv_mul;
@@ -410,7 +440,7 @@ paged_prefill_kernel(PrefillParams p) {
 
     // ---- staging ----
     int page[NC];
-    u4 kr[NC], vr[NC];
+    u4 kr[NC][NL], vr[NC][NL];
     unsigned lost = 0;  // bit 2i: chunk i's page is bad; bit 2i + 1: it lies behind the end
     const auto key_of = [&](int st, int i) { return st * KS + (tid + i * NT) / CH; };
     const auto look_up = [&](int st) {
@@ -428,23 +458,41 @@ paged_prefill_kernel(PrefillParams p) {
             if (u >= vis.count) lost |= 2u << (2 * i);
             const int t = vis.row(min(u, vis.count - 1));
             const T* at = pages + paged_at(b, ok ? page[i] : 0, 0, g, t & slot_mask, HD) +
-                          (tid + i * NT) % CH * CV;
-            kr[i] = *reinterpret_cast<const u4*>(at);
-            vr[i] = *reinterpret_cast<const u4*>(at + to_v);
+                          (tid + i * NT) % CH * 8;
+#pragma unroll
+            for (int e = 0; e < NL; ++e) {
+                kr[i][e] = reinterpret_cast<const u4*>(at)[e];
+                vr[i][e] = reinterpret_cast<const u4*>(at + to_v)[e];
+            }
         }
     };
     // Into LDS.  Rows behind the end are zeros; of a bad page K is NaN, so that
-    // the scores of the rows that see it are.  Whether V holds a value that is
-    // not finite is asked for where some rows do not see it (ask).
-    bool odd = false;
-    const auto stage = [&](int buf, bool ask) {
+    // the scores of the rows that see it are.
+    Range<T> range;
+    const auto put = [&](u4* at, int plane, const u4 (&x)[NL]) {
+        if constexpr (BF) {
+            *at = x[0];
+        } else {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(x[e / 4][e % 4]);
+            bf8 w[3];
+            split8(f, w);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) at[k * plane] = __builtin_bit_cast(u4, w[k]);
+        }
+    };
+    const auto stage = [&](int buf) {
         if (__any(lost != 0)) {
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 if (lost & (3u << (2 * i))) {
                     const unsigned w = lost & (2u << (2 * i)) ? 0u : BF ? 0x7FC07FC0u : 0x7FC00000u;
-                    kr[i] = u4{w, w, w, w};
-                    vr[i] = u4{0, 0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < NL; ++e) {
+                        kr[i][e] = u4{w, w, w, w};
+                        vr[i][e] = u4{0, 0, 0, 0};
+                    }
                 }
             }
         }
@@ -452,18 +500,21 @@ paged_prefill_kernel(PrefillParams p) {
         for (int i = 0; i < NC; ++i) {
             const int e = tid + i * NT, row = e / CH;
             if (!EXACT && row >= KS) break;
-            s_k[buf * KS * KST + row * KST + e % CH] = kr[i];
-            s_v[buf * KS * VST + row * VST + e % CH] = vr[i];
-            if (ask) odd |= not_finite<T>(vr[i]);
+#pragma unroll
+            for (int h = 0; h < NL; ++h) {
+                range.add(vr[i][h]);
+                if (!BF) range.add(kr[i][h]);
+            }
+            put(s_k + (buf * NP * KS + row) * KST + e % CH, KS * KST, kr[i]);
+            put(s_v + (buf * NP * KS + row) * VST + e % CH, KS * VST, vr[i]);
         }
     };
 
     // ---- q ----
     // Lane (n, half) holds dims 16 i + 8 half + (0..7) of packed row n, times a
-    // power of two for bf16 pages.
+    // power of two, in three planes.
     float scale = p.scale_log2;
-    bf8 qb[BF ? NQ : 1][3];
-    float qf[BF ? 1 : NQ][8];
+    bf8 qb[NQ][3];
     {
         // the first pages' ids are asked for first, then q, then the first keys
         const bool any = st_beg < st_end;
@@ -481,34 +532,27 @@ paged_prefill_kernel(PrefillParams p) {
             fetch(st_beg);
             if (st_beg + 1 < st_end) look_up(st_beg + 1);
         }
-        if constexpr (BF) {
-            float top = 0.0f;
+        float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NQ; ++i)
+        for (int i = 0; i < NQ; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(xq[i][e]));
-            top = fmaxf(top, other_half(top));
-            // largest magnitude in [2^-8, 2^-7): sums of hd products with any
-            // bf16 K stay finite
-            int ex = 0;
-            if (top > 0.0f && top < INFINITY) {
-                (void)frexpf(top, &ex);
-                ex += 7;
-            }
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) xq[i][e] = ldexpf(xq[i][e], -ex);
-                split8(xq[i], qb[i]);
-            }
-            // (never 0: scores of -inf must stay -inf)
-            scale = fmaxf(ldexpf(scale, ex), FLT_MIN);
-        } else {
-#pragma unroll
-            for (int i = 0; i < NQ; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) qf[i][e] = xq[i][e];
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(xq[i][e]));
+        top = fmaxf(top, other_half(top));
+        // largest magnitude in [2^-8, 2^-7): sums of hd products with any bf16 K
+        // stay finite
+        int ex = 0;
+        if (top > 0.0f && top < INFINITY) {
+            (void)frexpf(top, &ex);
+            ex += 7;
         }
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) xq[i][e] = ldexpf(xq[i][e], -ex);
+            split8(xq[i], qb[i]);
+        }
+        // (never 0: scores of -inf must stay -inf)
+        scale = fmaxf(ldexpf(scale, ex), FLT_MIN);
     }
 
     v16 o[ND];
@@ -517,28 +561,23 @@ paged_prefill_kernel(PrefillParams p) {
     float m = -FLT_MAX, l = 0.0f;  // finite m: a row that has seen no key yet needs no guard
 
     // ---- one tile of the wave ----
+    // The products of planes (K or V, q or p), small ones first.
+    constexpr int NPR = BF ? 3 : 6;
+    constexpr int PA[6] = {BF ? 0 : 2, 0, BF ? 0 : 1, 1, 0, 0};
+    constexpr int PB[6] = {BF ? 2 : 0, BF ? 1 : 2, BF ? 0 : 1, 0, 1, 0};
     const auto attend = [&](int buf, int u0) {
-        const u4* sk = s_k + (buf * KS + ksp * KT) * KST;
-        const u4* sv = s_v + (buf * KS + ksp * KT) * VST;
+        const u4* sk = s_k + (buf * NP * KS + ksp * KT) * KST;
+        const u4* sv = s_v + (buf * NP * KS + ksp * KT) * VST;
         v16 s = v16{};
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
-            if constexpr (BF) {
-                const bf8 kf = __builtin_bit_cast(bf8, sk[n * KST + 2 * i + half]);
+            bf8 kf[NP];
 #pragma unroll
-                for (int k = 2; k >= 0; --k)
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[i][k], s, 0, 0, 0);
-            } else {
-                // dims 16 i + 8 half + (0..7), as q has them
+            for (int k = 0; k < NP; ++k)
+                kf[k] = __builtin_bit_cast(bf8, sk[k * KS * KST + n * KST + 2 * i + half]);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const u4 kf = sk[n * KST + 4 * i + 2 * half + c];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(kf[e]),
-                                                                 qf[i][4 * c + e], s, 0, 0, 0);
-                }
-            }
+            for (int e = 0; e < NPR; ++e)
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[PA[e]], qb[i][PB[e]], s, 0, 0, 0);
         }
         // Rows u0 .. u0 + 31 are t0 .. t0 + 31, or they lie on both sides of
         // the gap, or behind the end (then t > pos for every row).
@@ -576,42 +615,36 @@ paged_prefill_kernel(PrefillParams p) {
         l += ps;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            if constexpr (BF) {
-                bf8 pf[3];
-                const float xs[8] = {s[8 * ks],     s[8 * ks + 1], s[8 * ks + 2], s[8 * ks + 3],
-                                     s[8 * ks + 4], s[8 * ks + 5], s[8 * ks + 6], s[8 * ks + 7]};
-                split8(xs, pf);
+            bf8 pf[3];
+            const float xs[8] = {s[8 * ks],     s[8 * ks + 1], s[8 * ks + 2], s[8 * ks + 3],
+                                 s[8 * ks + 4], s[8 * ks + 5], s[8 * ks + 6], s[8 * ks + 7]};
+            split8(xs, pf);
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    // 16 lanes read a 4 x 16 block row by row and get it column
-                    // by column; dims behind HD repeat others
-                    const int dim = DPAD && d == ND - 1 ? 4 * (lane & 3)
-                                                        : 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+            for (int d = 0; d < ND; ++d) {
+                // 16 lanes read a 4 x 16 block row by row and get it column by
+                // column; dims behind HD repeat others
+                const int dim = DPAD && d == ND - 1 ? 4 * (lane & 3)
+                                                    : 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+                bf8 vf[NP];
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
                     s4 w[2];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const int row = 16 * ks + 8 * c + 4 * half + ((lane >> 2) & 3);
-                        const T* at = reinterpret_cast<const T*>(&sv[row * VST]) + 32 * d + dim;
+                        const short* at =
+                            reinterpret_cast<const short*>(sv + k * KS * VST + row * VST) + 32 * d +
+                            dim;
                         w[c] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (__attribute__((address_space(3))) s4*)(at));
                     }
                     const u2 w0 = __builtin_bit_cast(u2, w[0]), w1 = __builtin_bit_cast(u2, w[1]);
-                    const bf8 vf = __builtin_bit_cast(bf8, u4{w0[0], w0[1], w1[0], w1[1]});
-#pragma unroll
-                    for (int k = 2; k >= 0; --k)
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[k], o[d], 0, 0, 0);
+                    vf[k] = __builtin_bit_cast(bf8, u4{w0[0], w0[1], w1[0], w1[1]});
                 }
-            } else {
 #pragma unroll
-                for (int d = 0; d < ND; ++d) {
-                    const int dim = 32 * d + (DPAD && d == ND - 1 ? n & 15 : n);
-#pragma unroll
-                    for (int r = 8 * ks; r < 8 * ks + 8; ++r) {
-                        const int row = 8 * (r / 4) + 4 * half + r % 4;
-                        const float v = reinterpret_cast<const float*>(&sv[row * VST])[dim];
-                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[r], o[d], 0, 0, 0);
-                    }
-                }
+                for (int e = 0; e < NPR; ++e)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[PA[e]], pf[PB[e]], o[d], 0, 0,
+                                                                   0);
             }
         }
     };
@@ -619,10 +652,8 @@ paged_prefill_kernel(PrefillParams p) {
     // ---- the steps ----
     if (st_beg < st_end) {  // uniform
         for (int st = st_beg; st < st_end; ++st) {
-            const int u = st * KS, t = vis.row(u), buf = NB == 2 ? st & 1 : 0;
-            // some row of the workgroup does not see some key of the step
-            const bool ask = u + KS > vis.count || t + KS - 1 > pos_first || p.window > 0;
-            stage(buf, ask);
+            const int u = st * KS, buf = NB == 2 ? st & 1 : 0;
+            stage(buf);
             if (st + 1 < st_end) {
                 fetch(st + 1);
                 if (st + 2 < st_end) look_up(st + 2);
@@ -636,9 +667,7 @@ paged_prefill_kernel(PrefillParams p) {
         }
     }
     l += other_half(l);
-    // an infinity or a NaN in V where some rows do not see it: 0 * inf is NaN
-    // in a product, so the rows are computed again, key by key
-    const bool redo = __syncthreads_or(odd);  // (and every wave is done with the tiles)
+    const bool redo = __syncthreads_or(range.outside());  // (and every wave is done with the tiles)
 
     // ---- key splits ----
     if constexpr (KSP > 1) {
@@ -807,26 +836,40 @@ hipError_t launch_k(const Shape& s, PrefillParams p, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Groups of packed rows and key splits of a workgroup.
+// Groups of packed rows and key splits of a workgroup, by wgs, the workgroups
+// that 128-row tiles make, and the keys of the longest row.  Four groups share
+// what is staged; key splits put eight waves on a CU that would have four, and
+// shorten the longest workgroup where there are few; a split over workgroups
+// (launch_k) costs a second launch, but needs no merge in LDS.  Measured over
+// 16 to 4096 rows behind 0 and 2000, page 32 (us):
+//   hd 128 bf16, 4 x 1 against 4 x 2: wgs 32, 128 keys 17.5 / 19.7; wgs 128 behind
+//     2000 94 / 79; wgs 512 143 / 121; wgs 1024 423 / 439
+//   hd 128 f32, 4 x 2 against 2 x 2: wgs 32, 128 keys 29.9 / 19.3; wgs 128 behind
+//     2000 177 / 192; 4 x 1 against 4 x 2 at wgs 512 behind 2000 718 / 780
+//   hd 64 bf16, 4 x 2, 2 x 4 and 1 x 8: wgs 18 17.1 / 14.3 / 13.3; wgs 72 behind
+//     2000 44.9 / 56.2 / 64.3; wgs 144 63.8 / 41.9 / 56.4
+//   hd 64 f32, 4 x 2 against 1 x 4: wgs 9 15.6 / 11.1; wgs 36 behind 2000 37.6 / 81.9
+//   hd 256 bf16, 4 x 1 against 2 x 2: wgs 4 28.8 / 22.3; wgs 64 78.4 / 84.6
 template <class T, int HD>
 hipError_t launch_t(const Shape& s, const PrefillParams& p, hipStream_t st) {
-    const long wgs = tiles_bound(p.b, s.kv_mul, 128) * s.num_kv_heads;  // with four groups
+    constexpr bool BF = sizeof(T) == 2;
+    const long wgs = tiles_bound(p.b, s.kv_mul, 128) * s.num_kv_heads;
     const long keys = keys_bound(p);
-    static const int ek = getenv("SLM_KSP") ? atoi(getenv("SLM_KSP")) : 0;  // TEMP
-    if (ek == 1) return launch_k<T, HD, 4, 1>(s, p, st);
-    if constexpr (HD <= 128) if (ek == 2) return launch_k<T, HD, 4, 2>(s, p, st);
     if constexpr (HD > 128) {
-        if (wgs <= s.cus / 8) return launch_k<T, HD, 2, 2>(s, p, st);
+        if constexpr (BF)
+            if (wgs <= s.cus / 8) return launch_k<T, HD, 2, 2>(s, p, st);
     } else if constexpr (HD > 64) {
-        if constexpr (sizeof(T) == 4) {
-            if (keys > 32 && wgs <= s.cus / 4 &&
-                (keys <= 512 || (long)p.b.n_rows * s.kv_mul <= 64L * p.b.n_seqs))
-                return launch_k<T, HD, 1, 4>(s, p, st);
-        }
-        if (keys > 128 && wgs < 3 * s.cus) return launch_k<T, HD, 4, 2>(s, p, st);
+        if constexpr (!BF)
+            if (keys > 32 && wgs <= (keys <= 1024 ? s.cus : s.cus / 8))
+                return launch_k<T, HD, 2, 2>(s, p, st);
+        if (wgs >= s.cus * 3 / 8 && wgs < (BF ? 3 : 2) * s.cus)
+            return launch_k<T, HD, 4, 2>(s, p, st);
     } else if (keys > 64) {
-        if (wgs <= s.cus * 5 / 16) return launch_k<T, HD, 1, 8>(s, p, st);
-        if (wgs <= s.cus * 5 / 8) return launch_k<T, HD, 2, 4>(s, p, st);
+        constexpr bool k8 = tile_bytes<T, HD, 8>() <= kLds;  // or four splits
+        if (wgs <= s.cus / (keys <= 1024 ? 4 : k8 ? 8 : 16))
+            return launch_k<T, HD, 1, k8 ? 8 : 4>(s, p, st);
+        if (wgs > s.cus / 2 - s.cus / 8 && wgs <= s.cus * 5 / 8)
+            return launch_k<T, HD, 2, 4>(s, p, st);
         if (wgs < 3 * s.cus) return launch_k<T, HD, 4, 2>(s, p, st);
     }
     return launch_k<T, HD, 4, 1>(s, p, st);
