@@ -21,4 +21,20 @@ __device__ __forceinline__ PagedRow paged_row_wave(const PagedView& b, int row) 
     return paged_row_of(b, below - 1, end, row);
 }
 
+// Sum over the lanes up to this one, in DPP steps: within the 16-lane rows, then
+// the last lane of a row to the next, then that of the first two to the others.
+__device__ __forceinline__ int wave_upto(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);  // row_shr:2
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);  // row_shr:4
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);  // row_shr:8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31
+    return x;
+}
+
+__device__ __forceinline__ int wave_total(int x) {
+    return __builtin_amdgcn_readlane(wave_upto(x), 63);
+}
+
 }  // namespace slm

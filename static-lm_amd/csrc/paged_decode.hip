@@ -14,9 +14,12 @@
 // Every wave therefore forms the same plan from them: with T_r the tiles of
 // row r's visible keys (one at least), T their sum and U the workgroups per KV
 // head group that fill the card, a chunk is C = ceil(T / U) tiles and row r has
-// ceil(T_r / C) chunks.  That is at most U + n_rows chunks whatever the lengths
-// are, which is the grid; workgroups behind the last chunk end at once.  A row
-// of one chunk is written to out directly.
+// ceil(T_r / C) chunks, at most U + n_rows together, which is the grid;
+// workgroups behind the last chunk end at once.  Where C would exceed
+// kLongChunk tiles, more and shorter chunks even out the CUs' loads: up to 4 U, of kChunk
+// tiles at least (64 sequences of up to 4201 rows, Llama-3-8B shape in bf16: 133
+// us with U, 110 us with 4 U; 16 of them 38.1 and 48.8).  A row of one chunk is
+// written to out directly.
 //
 // Lanes.  LPG lanes hold one key's head_dim values in 16-byte loads, so a wave
 // attends 64 / LPG keys at a time, each lane group with its own (m, l, o); the
@@ -24,6 +27,8 @@
 // window's gap (Visible), and each lane group looks its page up a tile ahead.
 #include <float.h>
 #include <math.h>
+
+#include <algorithm>
 
 #include "paged_common.h"
 #include "slm_internal.h"
@@ -76,7 +81,11 @@ template <> struct Cfg<__bf16, 128> { static constexpr int LPG = 16, TP = 4; };
 template <> struct Cfg<__bf16, 256> { static constexpr int LPG = 32, TP = 4; };
 
 constexpr int kWaves = 4;
+constexpr int kXcds = 8;
 constexpr int kMaxGb = 4;  // query heads of a workgroup, at most
+// Tiles up to which no row is split: a tile costs its workgroup about 1 us, the
+// second launch that joins chunks 4.
+constexpr int kWholeTiles = 4;
 
 template <class T, int HD>
 constexpr int tile_rows() {
@@ -90,6 +99,7 @@ struct DecodeParams {
     float* part_o;    // [chunk][num_heads][head_dim]
     float* part_ml;   // [chunk][num_heads][2]
     int units;        // U, chunks to aim for; 0: every row is one chunk
+    int most_units;   // and where they would exceed kChunk tiles
     int num_heads;
     int kv_mul;
     int gb;           // query heads of a workgroup
@@ -98,13 +108,14 @@ struct DecodeParams {
     float scale_log2;
 };
 
-__device__ __forceinline__ long long wave_sum_ll(long long x) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+// Where chunk `want` of the batch (or the first chunk of row `row_want`) lies.
+constexpr int kChunk = 8, kLongChunk = 16;
+
+__device__ __forceinline__ int chunk_tiles(const DecodeParams& p, int total) {  // (0 < total < 2^30)
+    const int c = (total + p.units - 1) / p.units;
+    return c <= kLongChunk ? c : max(kChunk, (total + p.most_units - 1) / p.most_units);
 }
 
-// Where chunk `want` (or the first chunk of row `row_want`) lies.
 struct Chunk {
     int row;     // -1: behind the last chunk
     int index;   // within its row
@@ -122,32 +133,34 @@ __device__ __forceinline__ int row_tiles(const DecodeParams& p, int row) {
 // Every lane of the wave gets the same answer.
 template <int TILE>
 __device__ Chunk find_chunk(const DecodeParams& p, int want, int row_want) {
-    const int lane = threadIdx.x & 63;
     const int n = p.b.n_rows;
-    int mine = lane < n ? row_tiles<TILE>(p, lane) : 0;
-    long long total = mine;
+    if (n == 1) {  // nothing to look for
+        const int t = row_tiles<TILE>(p, 0), c = chunk_tiles(p, t);
+        const int k = (t + c - 1) / c;
+        return Chunk{want < k ? 0 : -1, want, k, c, 0};
+    }
+    const int lane = threadIdx.x & 63;
+    const int mine0 = lane < n ? row_tiles<TILE>(p, lane) : 0;
+    int total = mine0;
     for (int r = lane + 64; r < n; r += 64) total += row_tiles<TILE>(p, r);
-    total = wave_sum_ll(total);
-    const int c = (int)((total + p.units - 1) / p.units);
+    const int c = __builtin_amdgcn_readfirstlane(chunk_tiles(p, wave_total(total)));
     int before = 0;  // chunks of the rows in front of this stretch of 64
     for (int r0 = 0; r0 < n; r0 += 64) {
-        if (r0) mine = r0 + lane < n ? row_tiles<TILE>(p, r0 + lane) : 0;
+        const int mine = !r0 ? mine0 : r0 + lane < n ? row_tiles<TILE>(p, r0 + lane) : 0;
         const int cnt = (mine + c - 1) / c;
-        int upto = cnt;  // chunks up to this lane's row
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(upto, o);
-            if (lane >= o) upto += y;
-        }
+        const int upto = wave_upto(cnt);  // chunks up to this lane's row
         const bool here = row_want >= 0 ? r0 + lane == row_want
                                         : lane + r0 < n && want < before + upto;
         const unsigned long long m = __ballot(here);
         if (m) {
             const int l = __ffsll(m) - 1;
-            const int k = __shfl(cnt, l), first = before + __shfl(upto, l) - k;
-            return Chunk{r0 + l, want - first, k, c, first};
+            const int k = __builtin_amdgcn_readlane(cnt, l);
+            const int first = before + __builtin_amdgcn_readlane(upto, l) - k;
+            return Chunk{__builtin_amdgcn_readfirstlane(r0 + l),
+                         __builtin_amdgcn_readfirstlane(want - first), k, c,
+                         __builtin_amdgcn_readfirstlane(first)};
         }
-        before += __shfl(upto, 63);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return Chunk{-1, 0, 0, c, 0};
 }
@@ -212,7 +225,8 @@ __device__ __forceinline__ void attend(const float (&q)[GB][NV][Vec<T>::N], cons
         }
 }
 
-template <class T, int HD, int GB>
+// REUSE: another workgroup reads the same keys for other heads.
+template <class T, int HD, int GB, bool REUSE>
 __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(DecodeParams p) {
     constexpr int LPG = Cfg<T, HD>::LPG, TP = Cfg<T, HD>::TP, N = Vec<T>::N;
     constexpr int NV = HD / LPG / N;
@@ -222,16 +236,24 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(DecodeParams 
     static_assert(HD % (LPG * N) == 0, "whole 16-byte loads");
     const PagedView& b = p.b;
 
+    // Workgroups go to the XCDs round-robin: the nhb that read the same keys for
+    // different heads are kXcds apart, so that one L2 serves them all, by plain
+    // loads (16 sequences of up to 4201 rows, 8 heads to the KV head at hd 128: f32
+    // 33.6 us side by side, 26.5 apart, 24.7 with plain loads; bf16 25.7, 24.7,
+    // 23.8).  Keys read once keep nontemporal loads (64 sequences, 4 heads: f32 185
+    // us against 202).
     const int nhb = (p.kv_mul + GB - 1) / GB;
-    const int groups = b.kv_heads * nhb;
-    const int idx = blockIdx.x / groups;
-    const int gy = blockIdx.x - idx * groups;
-    const int g = gy / nhb;
-    const int hb = (gy - g * nhb) * GB;  // this workgroup's heads in the KV head's kv_mul
+    const int eight = blockIdx.x / kXcds;
+    const int pair = eight / nhb * kXcds + blockIdx.x % kXcds;  // of a chunk and a KV head
+    const int idx = pair / b.kv_heads;
+    const int g = pair - idx * b.kv_heads;
+    const int hb = eight % nhb * GB;  // this workgroup's heads in the KV head's kv_mul
     const int h0 = g * p.kv_mul + hb;
 
     Chunk ch{idx, 0, 1, 0, 0};
-    if (p.units) {
+    if (!p.units) {
+        if (idx >= b.n_rows) return;
+    } else {
         ch = find_chunk<TILE>(p, idx, -1);
         if (ch.row < 0) return;
     }
@@ -292,8 +314,13 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(DecodeParams 
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
                 const T* a = at + N * (v * LPG + li);
-                kr[tp][v] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a));
-                vr[tp][v] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a + to_v));
+                if constexpr (REUSE) {
+                    kr[tp][v] = *reinterpret_cast<const u4*>(a);
+                    vr[tp][v] = *reinterpret_cast<const u4*>(a + to_v);
+                } else {
+                    kr[tp][v] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a));
+                    vr[tp][v] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a + to_v));
+                }
             }
         }
         if (tb + TILE < u_end) look_up(tb + TILE);
@@ -373,61 +400,84 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(DecodeParams 
     }
 }
 
-// Joins a row's chunks for one head: a workgroup per (row, head), R rows of
-// threads over the chunks.
+// Joins a row's chunks for one head: a workgroup per (row, head).  Lane groups of
+// HD / 4 lanes go through every R-th chunk each, four at a time in flight, with a
+// running max; their states are added through LDS in order.
 template <class T, int HD>
 __global__ __launch_bounds__(256) void paged_join_kernel(DecodeParams p) {
     constexpr int TILE = tile_rows<T, HD>();
-    constexpr int R = 256 / HD;  // chunks side by side
-    __shared__ float s_o[R][HD], s_l[R], s_m[4];
+    constexpr int L4 = HD / 4, R = 256 / L4, B = 4;
+    __shared__ float s_m[R], s_l[R];
+    __shared__ __align__(16) float s_o[R][HD];
     const int row = blockIdx.x / p.num_heads;
     const int h = blockIdx.x - row * p.num_heads;
     const Chunk ch = find_chunk<TILE>(p, 0, row);
     if (ch.count == 1) return;  // written by its workgroup
     const int t = threadIdx.x;
+    const int k = t / L4, d = t - k * L4;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-    float mx = -FLT_MAX;
-    for (int c = t; c < ch.count; c += 256)
-        mx = fmaxf(mx, ml[(size_t)(ch.first + c) * p.num_heads + h].x);
-    mx = wave_max(mx);
-    if ((t & 63) == 0) s_m[t >> 6] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    const int k = t / HD, d = t - k * HD;
     if (k < R) {
-        float so = 0.0f, sl = 0.0f;
-        for (int c = k; c < ch.count; c += R) {
-            const size_t at = (size_t)(ch.first + c) * p.num_heads + h;
-            const float2 x = ml[at];
-            const float e = fast_exp2(x.x - mx);
-            sl += e * x.y;
-            so += e * p.part_o[at * HD + d];
+        float m = -FLT_MAX, l = 0.0f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c0 = k; c0 < ch.count; c0 += B * R) {
+            float2 y[B];
+            float4 z[B];
+#pragma unroll
+            for (int i = 0; i < B; ++i) {  // behind the last chunk: the last once more
+                const size_t at =
+                    (size_t)(ch.first + min(c0 + i * R, ch.count - 1)) * p.num_heads + h;
+                y[i] = ml[at];
+                z[i] = ld4(p.part_o + at * HD + 4 * d);
+            }
+            float mn = m;
+#pragma unroll
+            for (int i = 0; i < B; ++i) mn = fmaxf(mn, y[i].x);
+            const float a = fast_exp2(m - mn);
+            m = mn;
+            l *= a;
+            o.x *= a, o.y *= a, o.z *= a, o.w *= a;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                if (c0 + i * R >= ch.count) break;
+                const float e = fast_exp2(y[i].x - m);
+                l = fmaf(e, y[i].y, l);
+                o.x = fmaf(e, z[i].x, o.x);
+                o.y = fmaf(e, z[i].y, o.y);
+                o.z = fmaf(e, z[i].z, o.z);
+                o.w = fmaf(e, z[i].w, o.w);
+            }
         }
-        s_o[k][d] = so;
-        if (d == 0) s_l[k] = sl;
+        if (d == 0) {
+            s_m[k] = m;
+            s_l[k] = l;
+        }
+        *reinterpret_cast<float4*>(&s_o[k][4 * d]) = o;
     }
     __syncthreads();
     if (t < HD) {
-        float so = s_o[0][t], sl = s_l[0];
-#pragma unroll
-        for (int i = 1; i < R; ++i) {
-            so += s_o[i][t];
-            sl += s_l[i];
+        const int n = min(R, ch.count);
+        float mx = s_m[0], so = 0.0f, sl = 0.0f;
+        for (int i = 1; i < n; ++i) mx = fmaxf(mx, s_m[i]);
+        for (int i = 0; i < n; ++i) {
+            const float e = fast_exp2(s_m[i] - mx);
+            sl = fmaf(e, s_l[i], sl);
+            so = fmaf(e, s_o[i][t], so);
         }
         p.out[((size_t)row * p.num_heads + h) * HD + t] = so / sl;
     }
+}
+
+// Query heads of a workgroup: kv_mul in equal parts of at most four (eight took
+// 1.3 to 2 times as long: half the waves fit).
+int gb_of(int kv_mul) {
+    const int parts = (kv_mul + kMaxGb - 1) / kMaxGb;
+    return (kv_mul + parts - 1) / parts;
 }
 
 // Workgroups per KV head group that fill the card with two waves per SIMD.
 int units_of(const Shape& s, int groups) {
     const int wgs = 2 * s.cus;
     return groups >= wgs ? 1 : wgs / groups;
-}
-
-// Query heads of a workgroup: kv_mul in equal parts of at most four.
-int gb_of(int kv_mul) {
-    const int parts = (kv_mul + kMaxGb - 1) / kMaxGb;
-    return (kv_mul + parts - 1) / parts;
 }
 
 int groups_of(const Shape& s) {
@@ -438,20 +488,32 @@ int groups_of(const Shape& s) {
 template <class T, int HD>
 hipError_t launch_t(const Shape& s, DecodeParams p, hipStream_t st) {
     const int groups = groups_of(s);
-    // no sequence has more tiles than this
-    const int most = (p.b.max_len + tile_rows<T, HD>() - 1) / tile_rows<T, HD>();
-    if (p.units && (long)most * p.b.n_rows < p.units) p.units = most * p.b.n_rows;
-    if (most == 1) p.units = 0;
-    const long wgs = ((long)p.units + p.b.n_rows) * groups;
-    if (wgs > (1L << 30) / 256 || (long)p.b.n_rows * s.num_heads > (1L << 30) / 256)
+    // no row has more tiles than this
+    const long keys = p.window > 0 ? std::min<long>(p.b.max_len, (long)p.window + p.sinks)
+                                   : p.b.max_len;
+    const long most = (keys + tile_rows<T, HD>() - 1) / tile_rows<T, HD>();
+    if (most <= kWholeTiles) p.units = 0;
+    const long all = most * p.b.n_rows;
+    p.units = (int)std::min<long>(p.units, all);
+    p.most_units = (int)std::max<long>(p.units, std::min<long>(4L * p.units, all / kChunk + 1));
+    const long pairs = ((long)p.most_units + p.b.n_rows) * s.num_kv_heads;
+    const long wgs = (pairs + kXcds - 1) / kXcds * kXcds * (groups / s.num_kv_heads);
+    if (all >= 1L << 30 || wgs > (1L << 30) / 256 || (long)p.b.n_rows * s.num_heads > (1L << 30) / 256)
         return hipErrorInvalidValue;
     const dim3 grid((unsigned)wgs);
-    switch (p.gb) {
-        case 1: hipLaunchKernelGGL((paged_decode_kernel<T, HD, 1>), grid, dim3(256), 0, st, p); break;
-        case 2: hipLaunchKernelGGL((paged_decode_kernel<T, HD, 2>), grid, dim3(256), 0, st, p); break;
-        case 3: hipLaunchKernelGGL((paged_decode_kernel<T, HD, 3>), grid, dim3(256), 0, st, p); break;
-        default: hipLaunchKernelGGL((paged_decode_kernel<T, HD, 4>), grid, dim3(256), 0, st, p);
-    }
+    const bool reuse = p.kv_mul > p.gb;  // of more than four heads: 3 or 4 of them
+    if (p.gb == 1)
+        hipLaunchKernelGGL((paged_decode_kernel<T, HD, 1, false>), grid, dim3(256), 0, st, p);
+    else if (p.gb == 2)
+        hipLaunchKernelGGL((paged_decode_kernel<T, HD, 2, false>), grid, dim3(256), 0, st, p);
+    else if (p.gb == 3 && !reuse)
+        hipLaunchKernelGGL((paged_decode_kernel<T, HD, 3, false>), grid, dim3(256), 0, st, p);
+    else if (p.gb == 3)
+        hipLaunchKernelGGL((paged_decode_kernel<T, HD, 3, true>), grid, dim3(256), 0, st, p);
+    else if (!reuse)
+        hipLaunchKernelGGL((paged_decode_kernel<T, HD, 4, false>), grid, dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((paged_decode_kernel<T, HD, 4, true>), grid, dim3(256), 0, st, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.units) return e;
     hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(p.b.n_rows * s.num_heads), dim3(256), 0,
@@ -476,7 +538,7 @@ hipError_t launch_hd(const Shape& s, const DecodeParams& p, hipStream_t st) {
 }  // namespace
 
 size_t paged_decode_chunks(const Shape& s, int max_rows) {
-    return (size_t)units_of(s, groups_of(s)) + max_rows;
+    return 4 * (size_t)units_of(s, groups_of(s)) + max_rows;
 }
 
 hipError_t launch_paged_decode(const Shape& s, const PagedView& b, bool bf16, const float* q,
@@ -484,7 +546,7 @@ hipError_t launch_paged_decode(const Shape& s, const PagedView& b, bool bf16, co
                                hipStream_t st) {
     const int gb = gb_of(s.kv_mul);
     const DecodeParams p{b,      q,     out,
-                         part_o, part_ml, part_o ? units_of(s, groups_of(s)) : 0,
+                         part_o, part_ml, units_of(s, groups_of(s)), 0,
                          s.num_heads, s.kv_mul, gb,
                          window, sinks, 1.4426950408889634f / sqrtf((float)s.head_dim)};
     return bf16 ? launch_hd<__bf16>(s, p, st) : launch_hd<float>(s, p, st);

@@ -210,12 +210,12 @@ __device__ Tile find_tile(const PrefillParams& p, int want, bool by_tile) {
         return Seq{lo, rows, len, (int)(((long long)rows * p.kv_mul + BM - 1) / BM),
                    max(1, (int)((keys + KS - 1) / KS))};
     };
-    const auto chunk_steps = [&](long long total) {
-        return p.units ? max(1, (int)((total + p.units - 1) / p.units)) : kUnsplit;
+    const auto chunk_steps = [&](int total) {
+        return p.units ? max(1, (total + p.units - 1) / p.units) : kUnsplit;
     };
     if (b.n_seqs == 1) {  // nothing to look for
         const Seq q = seq_of(0);
-        const int c = chunk_steps((long long)q.tiles * q.steps);
+        const int c = chunk_steps(q.tiles * q.steps);
         const int k = (q.steps + c - 1) / c, items = q.tiles * k;
         const int at = (by_tile ? q.tiles : items) - 1 - want;
         const int index = by_tile ? at : at / k;
@@ -231,29 +231,19 @@ __device__ Tile find_tile(const PrefillParams& p, int want, bool by_tile) {
     const Seq q0 = mine(b.n_seqs);
     int c = kUnsplit;
     if (p.units) {
-        long long total = (long long)q0.tiles * q0.steps;
+        int total = q0.tiles * q0.steps;
         for (int top = b.n_seqs - 64; top > 0; top -= 64) {
             const Seq q = mine(top);
-            total += (long long)q.tiles * q.steps;
+            total += q.tiles * q.steps;
         }
-#pragma unroll
-        for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
-        c = chunk_steps(total);
+        c = chunk_steps(wave_total(total));
     }
-    const auto upto = [&](int x) {  // sum over the lanes up to this one
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(x, o);
-            if (lane >= o) x += y;
-        }
-        return x;
-    };
     int before = 0, items_before = 0;
     for (int top = b.n_seqs; top > 0; top -= 64) {
         const Seq q = top == b.n_seqs ? q0 : mine(top);
         const int k = (q.steps + c - 1) / c;
-        const int items = upto(q.tiles * k);
-        const int cnt = by_tile ? upto(q.tiles) : items;
+        const int items = wave_upto(q.tiles * k);
+        const int cnt = by_tile ? wave_upto(q.tiles) : items;
         const unsigned long long m = __ballot(want < before + cnt);
         if (m) {
             const int l = __ffsll(m) - 1;
@@ -824,6 +814,8 @@ hipError_t launch_k(const Shape& s, PrefillParams p, hipStream_t st) {
     const long ns = s.cus / (tiles * s.num_kv_heads);
     const long steps = (keys_bound(p) + KS - 1) / KS;
     p.units = ns >= 2 && steps * (ns - 1) >= 4 * ns ? (int)(ns * tiles) : 0;
+    // (the plan's sums are 32-bit, also of row starts that overlap)
+    if (tiles * steps * p.b.n_seqs >= 1L << 30) p.units = 0;
     const long wgs = (tiles + p.units) * s.num_kv_heads;
     if (wgs >= (1L << 32) / NT) return hipErrorInvalidValue;
     hipLaunchKernelGGL((paged_prefill_kernel<T, HD, RG, KSP>), dim3((unsigned)wgs), dim3(NT), 0, st,

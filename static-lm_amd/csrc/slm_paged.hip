@@ -86,6 +86,9 @@ int check_call(slm_attn_ctx* c, const slm_paged_cache* cache, int layer,
     // workgroups of 256 threads are counted in 24 bits
     if ((int64_t)b->n_rows * s.num_heads + (int64_t)b->n_seqs * s.num_kv_heads >= INT64_C(1) << 23)
         return fail(c, SLM_ERR_BATCH, "too many rows and heads in one call (2^23)");
+    // the split decode adds up the sequences' tiles of 16 rows or more in 32 bits
+    if ((int64_t)b->n_seqs * (b->max_len / 16 + 1) >= INT64_C(1) << 30)
+        return fail(c, SLM_ERR_BATCH, "n_seqs * max_len must be below 2^34");
     return SLM_OK;
 }
 
