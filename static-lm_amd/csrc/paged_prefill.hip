@@ -206,7 +206,7 @@ __device__ Tile find_tile(const PrefillParams& p, int want, bool by_tile) {
         const int rows = paged_min(paged_max(b.row_start[s + 1], lo), b.n_rows) - lo;
         const int len = b.lens[s];
         long long keys = len < 0 || len > b.max_len ? 0 : len;
-        if (p.window > 0) keys = min(keys, (long long)p.window + p.sinks + BM / p.kv_mul + 2);
+        if (p.window > 0) keys = min(keys, (long long)p.window + p.sinks + BM / p.kv_mul + 2 + 2 * KT);
         return Seq{lo, rows, len, (int)(((long long)rows * p.kv_mul + BM - 1) / BM),
                    max(1, (int)((keys + KS - 1) / KS))};
     };
@@ -266,6 +266,16 @@ __device__ Tile find_tile(const PrefillParams& p, int want, bool by_tile) {
     return Tile{-1, 0, 0, 0, 0, 0, 0, 0};
 }
 
+// find_tile's answer in scalar registers (the compiler does not see that every
+// lane has the same).
+template <int BM, int KS>
+__device__ __forceinline__ Tile find_tile_uniform(const PrefillParams& p, int want, bool by_tile) {
+    const auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const Tile t = find_tile<BM, KS>(p, want, by_tile);
+    return Tile{u(t.seq), u(t.index), u(t.row0),  u(t.rows),
+                u(t.len), u(t.chunk), u(t.steps), u(t.item0)};
+}
+
 // Where a tile lies, and the keys that any of its rows sees: Visible of the
 // last row, from the first row's window on.
 template <int BM, int KS>
@@ -288,8 +298,8 @@ struct Span {
         pos_last = pos0 + (min(x0 + BM, packed) - 1) / p.kv_mul;
         vis = Visible(pos_last, 0, 0);
         if (pos_last >= 0 && p.window > 0) {
-            vis.lo = max(0, pos_first + 1 - p.window);
-            vis.first = min(p.sinks, vis.lo);
+            vis.lo = max(0, pos_first + 1 - p.window) / KT * KT;
+            vis.first = min((min(p.sinks, vis.lo) + KT - 1) / KT * KT, vis.lo);
             vis.count = vis.first + pos_last + 1 - vis.lo;
         }
         steps = (vis.count + KS - 1) / KS;
@@ -302,10 +312,11 @@ struct Span {
 // a key per lane, then the sum with dims over the lanes, in which a key that the
 // row does not see has no part.  For the rare tile whose K or V the matrix cores
 // cannot take.  The state goes to m, l and o of the row: into out, or the
-// partials of row `part` + x.
+// partials of row `part` + x.  (Arguments by value: of a reference the caller's
+// copy would live in memory, in its hot loop as well.)
 template <class T, int HD>
-__device__ __noinline__ void attend_again(const PrefillParams& p, const Tile& tile, int g,
-                                          const Visible& vis, int u_beg, int u_end, int x, int end,
+__device__ __noinline__ void attend_again(const PrefillParams p, const Tile tile, int g,
+                                          const Visible vis, int u_beg, int u_end, int x, int end,
                                           int step, int pos0, bool bad, bool whole, size_t part) {
     constexpr int NL = (HD + 63) / 64;  // dims of a lane
     const PagedView& b = p.b;
@@ -402,7 +413,7 @@ paged_prefill_kernel(PrefillParams p) {
 
     const int g = blockIdx.x % b.kv_heads;
     const int item = blockIdx.x / b.kv_heads;
-    const Tile tile = find_tile<BM, KS>(p, item, false);
+    const Tile tile = find_tile_uniform<BM, KS>(p, item, false);
     if (tile.seq < 0) return;  // uniform
     const Span<BM, KS> span(p, tile);
     if (tile.chunk >= span.chunks) return;
@@ -429,30 +440,54 @@ paged_prefill_kernel(PrefillParams p) {
     const size_t to_v = ((size_t)b.kv_heads << b.ps_shift) * HD;
 
     // ---- staging ----
+    // Chunk e of a step is chunk e % CH of its row e / CH; a thread has e = tid,
+    // tid + NT, ..  Where the 64 chunks of a wave are whole rows of one page
+    // (UNI), the page is looked up and the address formed by the scalar unit.
+    constexpr bool UNI = CH >= 4 && (CH & (CH - 1)) == 0;
+    const int pos_last = span.pos_last;
     int page[NC];
     u4 kr[NC][NL], vr[NC][NL];
-    unsigned lost = 0;  // bit 2i: chunk i's page is bad; bit 2i + 1: it lies behind the end
+    // UNI: bit i: the page of chunk i is bad.  Else bit 2i: that, and bit 2i + 1:
+    // it lies behind the end.
+    unsigned lost = 0;
     const auto key_of = [&](int st, int i) { return st * KS + (tid + i * NT) / CH; };
+    const auto first_row = [&](int st, int i) {  // of the wave's chunks i (uniform)
+        const int row = (wave * 64 + i * NT) / CH;
+        return vis.row(st * KS + row / KT * KT) + row % KT;
+    };
     const auto look_up = [&](int st) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-            page[i] = table[vis.row(min(key_of(st, i), vis.count - 1)) >> b.ps_shift];
+        for (int i = 0; i < NC; ++i) {
+            if constexpr (UNI)
+                page[i] = ((const __attribute__((address_space(4))) int32_t*)
+                               table)[min(first_row(st, i), pos_last) >> b.ps_shift];
+            else
+                page[i] = table[vis.row(min(key_of(st, i), vis.count - 1)) >> b.ps_shift];
+        }
     };
     const auto fetch = [&](int st) {
         lost = 0;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int u = key_of(st, i);
             const bool ok = paged_page_ok(b, page[i]);
-            if (!ok) lost |= 1u << (2 * i);
-            if (u >= vis.count) lost |= 2u << (2 * i);
-            const int t = vis.row(min(u, vis.count - 1));
-            const T* at = pages + paged_at(b, ok ? page[i] : 0, 0, g, t & slot_mask, HD) +
-                          (tid + i * NT) % CH * 8;
+            const T* at;
+            if constexpr (UNI) {
+                if (!ok) lost |= 1u << i;
+                at = pages +
+                     paged_at(b, ok ? page[i] : 0, 0, g, first_row(st, i) & slot_mask, HD) +
+                     lane * 8;
+            } else {
+                const int u = key_of(st, i);
+                if (!ok) lost |= 1u << (2 * i);
+                if (u >= vis.count) lost |= 2u << (2 * i);
+                const int t = vis.row(min(u, vis.count - 1));
+                at = pages + paged_at(b, ok ? page[i] : 0, 0, g, t & slot_mask, HD) +
+                     (tid + i * NT) % CH * 8;
+            }
 #pragma unroll
             for (int e = 0; e < NL; ++e) {
-                kr[i][e] = reinterpret_cast<const u4*>(at)[e];
-                vr[i][e] = reinterpret_cast<const u4*>(at + to_v)[e];
+                kr[i][e] = ((const __attribute__((address_space(1))) u4*)at)[e];
+                vr[i][e] = ((const __attribute__((address_space(1))) u4*)(at + to_v))[e];
             }
         }
     };
@@ -472,19 +507,27 @@ paged_prefill_kernel(PrefillParams p) {
             for (int k = 0; k < 3; ++k) at[k * plane] = __builtin_bit_cast(u4, w[k]);
         }
     };
-    const auto stage = [&](int buf) {
-        if (__any(lost != 0)) {
+    const auto stage = [&](int st, int buf) {
+        const auto set = [&](int i, bool behind) {
+            const unsigned w = behind ? 0u : BF ? 0x7FC07FC0u : 0x7FC00000u;
+#pragma unroll
+            for (int e = 0; e < NL; ++e) {
+                kr[i][e] = u4{w, w, w, w};
+                vr[i][e] = u4{0, 0, 0, 0};
+            }
+        };
+        if constexpr (UNI) {
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
-                if (lost & (3u << (2 * i))) {
-                    const unsigned w = lost & (2u << (2 * i)) ? 0u : BF ? 0x7FC07FC0u : 0x7FC00000u;
-#pragma unroll
-                    for (int e = 0; e < NL; ++e) {
-                        kr[i][e] = u4{w, w, w, w};
-                        vr[i][e] = u4{0, 0, 0, 0};
-                    }
-                }
+                const int t = first_row(st, i);
+                if (lost >> i & 1) set(i, false);
+                if (t + 64 / CH - 1 > pos_last)  // uniform
+                    if (t + lane / CH > pos_last) set(i, true);
             }
+        } else if (__any(lost != 0)) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (lost & (3u << (2 * i))) set(i, lost & (2u << (2 * i)));
         }
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
@@ -569,17 +612,13 @@ paged_prefill_kernel(PrefillParams p) {
             for (int e = 0; e < NPR; ++e)
                 s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[PA[e]], qb[i][PB[e]], s, 0, 0, 0);
         }
-        // Rows u0 .. u0 + 31 are t0 .. t0 + 31, or they lie on both sides of
-        // the gap, or behind the end (then t > pos for every row).
+        // the tile's rows are t0 .. t0 + 31; some behind the end (t > every pos)
         const int t0 = vis.row(u0);
-        const bool gap = u0 < vis.first && u0 + KT > vis.first;
-        const bool hidden = gap || t0 + KT - 1 > wpos_first ||
-                            (p.window > 0 && u0 >= vis.first && t0 <= wpos_last - p.window);
-        if (hidden) {  // uniform
+        if (t0 + KT - 1 > wpos_first ||
+            (p.window > 0 && t0 <= wpos_last - p.window && t0 + KT > p.sinks)) {  // uniform
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int u = u0 + 8 * (r / 4) + 4 * half + r % 4;
-                const int t = u + (u < vis.first ? 0 : vis.lo - vis.first);
+                const int t = t0 + 8 * (r / 4) + 4 * half + r % 4;
                 const bool hide = (t > pos) | ((t <= pos_out) & (t >= p.sinks));
                 s[r] = hide ? -INFINITY : s[r];
             }
@@ -643,7 +682,7 @@ paged_prefill_kernel(PrefillParams p) {
     if (st_beg < st_end) {  // uniform
         for (int st = st_beg; st < st_end; ++st) {
             const int u = st * KS, buf = NB == 2 ? st & 1 : 0;
-            stage(buf);
+            stage(st, buf);
             if (st + 1 < st_end) {
                 fetch(st + 1);
                 if (st + 2 < st_end) look_up(st + 2);
@@ -743,7 +782,8 @@ __global__ __launch_bounds__(kThreads) void paged_prefill_join_kernel(PrefillPar
     constexpr int PARTS = (BM * HD / 4 + kThreads - 1) / kThreads;  // workgroups of a tile
     const PagedView& b = p.b;
     const int part = blockIdx.x % PARTS, g = blockIdx.x / PARTS % b.kv_heads;
-    const Tile tile = find_tile<BM, KS>(p, blockIdx.x / (PARTS * b.kv_heads), true);
+    const Tile tile =
+        find_tile_uniform<BM, KS>(p, blockIdx.x / (PARTS * b.kv_heads), true);
     if (tile.seq < 0) return;
     const Span<BM, KS> span(p, tile);
     if (span.chunks == 1) return;  // written by its workgroup
