@@ -46,10 +46,14 @@ typedef struct slm_paged_cache slm_paged_cache;
 
 /* A cache for the heads and on the device of `ctx`, whose RoPE tables and
  * stream its calls use; only that context may be given with it.  The pool is
- * zeroed; it and the workspace of the split decode (a few megabytes) are the
- * cache's until slm_paged_destroy.  Call that when the work that uses the
- * cache has finished (slm_attn_sync), before or after the context's own
- * destruction.  SLM_ERR_CONFIG for a value out of its range. */
+ * zeroed; it and the workspace for rows that are split over workgroups are the
+ * cache's until slm_paged_destroy.  (The workspace has 65536 rows of head_dim + 2
+ * floats, or num_heads * max_seqs + 8192 if that is more: 34 MB for 32 heads of
+ * 128 and up to 1792 sequences.)  Calls and replayed graphs with one cache
+ * share its rows and workspace: a program that moves its context to another
+ * stream orders the two.  Destroy a cache when the work that uses it has
+ * finished (slm_attn_sync), before or after the context's own destruction.
+ * SLM_ERR_CONFIG for a value out of its range. */
 int slm_paged_create(slm_attn_ctx* ctx, const slm_paged_config* cfg, slm_paged_cache** out);
 void slm_paged_destroy(slm_paged_cache* cache);
 
@@ -114,7 +118,8 @@ int slm_paged_append_dev(slm_attn_ctx* ctx, slm_paged_cache* cache, int32_t laye
  * sinks has no effect.  Scores are q . k / sqrt(head_dim); all sums and the
  * softmax are in f32.  A sequence's result depends on the other sequences of
  * the call by rounding only (they decide where its rows are split); the same
- * batch gives the same bits.  Visible rows of K must be finite. */
+ * batch gives the same bits.  Visible rows of K must be finite.  Runs of rows
+ * over bf16 pages take K values below 2^-90 with fewer digits, or as 0. */
 int slm_paged_attend_dev(slm_attn_ctx* ctx, slm_paged_cache* cache, int32_t layer,
                          const slm_paged_batch* batch, const float* q_rot, int32_t window,
                          int32_t sinks, float* out);

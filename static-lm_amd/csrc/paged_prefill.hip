@@ -28,7 +28,7 @@
 // two per row, so that values of any size stay within bf16's exponents; the
 // scores' scale takes it back.  What cannot be split or must not be multiplied
 // (V from 2^64 on, infinities and NaN among them; with f32 pages also K, and
-// values between 0 and 2^-100, whose remainders run out of exponents) makes the
+// values between 0 and 2^-96, whose remainders run out of exponents) makes the
 // workgroup compute its rows again in plain f32 (attend_again).
 //
 // What bounds it: the matrix cores for long runs, the softmax and the splitting
@@ -171,7 +171,7 @@ struct Range<float> {
         }
     }
     __device__ __forceinline__ bool outside() const {
-        return top >= 0x5F800000u || low < 0x0D800000u - 1;  // 2^64, 2^-100
+        return top >= 0x5F800000u || low < 0x0F800000u - 1;  // 2^64, 2^-96
     }
 };
 
@@ -544,9 +544,9 @@ paged_prefill_kernel(PrefillParams p) {
     };
 
     // ---- q ----
-    // Lane (n, half) holds dims 16 i + 8 half + (0..7) of packed row n, times a
-    // power of two, in three planes.
-    float scale = p.scale_log2;
+    // Lane (n, half) holds dims 16 i + 8 half + (0..7) of packed row n, times
+    // log2(e) / sqrt(hd) and a power of two, in three planes.
+    float scale;  // what takes the power back: the fused scale and max below are exact
     bf8 qb[NQ][3];
     {
         // the first pages' ids are asked for first, then q, then the first keys
@@ -559,7 +559,7 @@ paged_prefill_kernel(PrefillParams p) {
             const float4 a = ld4(src + 16 * i), c = ld4(src + 16 * i + 4);
             const float v[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) xq[i][e] = v[e];
+            for (int e = 0; e < 8; ++e) xq[i][e] = v[e] * p.scale_log2;
         }
         if (any) {
             fetch(st_beg);
@@ -571,12 +571,12 @@ paged_prefill_kernel(PrefillParams p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(xq[i][e]));
         top = fmaxf(top, other_half(top));
-        // largest magnitude in [2^-8, 2^-7): sums of hd products with any bf16 K
+        // largest magnitude in [2^-10, 2^-9): sums of 256 products with any bf16 K
         // stay finite
         int ex = 0;
         if (top > 0.0f && top < INFINITY) {
             (void)frexpf(top, &ex);
-            ex += 7;
+            ex += 9;
         }
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
@@ -584,8 +584,8 @@ paged_prefill_kernel(PrefillParams p) {
             for (int e = 0; e < 8; ++e) xq[i][e] = ldexpf(xq[i][e], -ex);
             split8(xq[i], qb[i]);
         }
-        // (never 0: scores of -inf must stay -inf)
-        scale = fmaxf(ldexpf(scale, ex), FLT_MIN);
+        // (never 0 or infinite: hidden scores must stay -inf, scores of 0 must stay 0)
+        scale = ldexpf(1.0f, min(max(ex, -126), 127));
     }
 
     v16 o[ND];

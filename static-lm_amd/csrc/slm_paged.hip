@@ -251,6 +251,9 @@ int slm_paged_attend_dev(slm_attn_ctx* c, slm_paged_cache* cache, int32_t layer,
     const size_t qb = (size_t)b->n_rows * s.dim * 4;
     if (overlaps(out, qb, q_rot, qb)) return fail(c, SLM_ERR_ALIAS, "out must not overlap q");
     if ((rc = check_written(c, cache, b, out, qb, "out"))) return rc;
+    // a window that hides nothing from any row is none (and the kernels' sums of
+    // positions and windows stay within 32 bits)
+    if ((int64_t)window + sinks >= b->max_len) window = 0;
     const slm::PagedView view = view_of(cache, layer, b);
     const OnDevice on(c->device);
     const bool bf16 = cache->cfg.dtype == SLM_PAGED_BF16;
