@@ -118,8 +118,8 @@ int slm_paged_append_dev(slm_attn_ctx* ctx, slm_paged_cache* cache, int32_t laye
  * sinks has no effect.  Scores are q . k / sqrt(head_dim); all sums and the
  * softmax are in f32.  A sequence's result depends on the other sequences of
  * the call by rounding only (they decide where its rows are split); the same
- * batch gives the same bits.  Visible rows of K must be finite.  Runs of rows
- * over bf16 pages take K values below 2^-90 with fewer digits, or as 0. */
+ * batch gives the same bits.  Visible rows of K must be finite.  K values
+ * of bf16 pages below 2^-90 may lose digits, or count as 0. */
 int slm_paged_attend_dev(slm_attn_ctx* ctx, slm_paged_cache* cache, int32_t layer,
                          const slm_paged_batch* batch, const float* q_rot, int32_t window,
                          int32_t sinks, float* out);

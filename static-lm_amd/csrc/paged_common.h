@@ -8,6 +8,38 @@
 
 namespace slm {
 
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+
+// Two values as bf16 pairs: x = p1 + p2 + p3 (24 bits).
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t* p1, uint32_t* p2,
+                                       uint32_t* p3) {
+    const auto pack = [](float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf2));
+    };
+    *p1 = pack(x0, x1);
+    x0 -= __uint_as_float(*p1 << 16);
+    x1 -= __uint_as_float(*p1 & 0xFFFF0000u);
+    *p2 = pack(x0, x1);
+    x0 -= __uint_as_float(*p2 << 16);
+    x1 -= __uint_as_float(*p2 & 0xFFFF0000u);
+    *p3 = pack(x0, x1);
+}
+
+__device__ __forceinline__ void split8(const float* x, bf8 (&p)[3]) {
+    u4 w[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t a, b, c;
+        split2(x[2 * i], x[2 * i + 1], &a, &b, &c);
+        w[0][i] = a, w[1][i] = b, w[2][i] = c;
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) p[k] = __builtin_bit_cast(bf8, w[k]);
+}
+
 // paged_row for a row that is the wave's (every lane of it is active): up to 63
 // sequences take one load of the starts and a ballot.
 __device__ __forceinline__ PagedRow paged_row_wave(const PagedView& b, int row) {

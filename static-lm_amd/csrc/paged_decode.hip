@@ -25,6 +25,9 @@
 // attends 64 / LPG keys at a time, each lane group with its own (m, l, o); the
 // states are merged through LDS at the end.  Keys are numbered without the
 // window's gap (Visible), and each lane group looks its page up a tile ahead.
+// With four query heads to a bf16 key the vector unit would be the bound: their
+// scores come from the matrix cores (matrix_scores), from q split into three
+// bf16 planes, which K needs not be.
 #include <float.h>
 #include <math.h>
 
@@ -36,8 +39,7 @@
 namespace slm {
 namespace {
 
-typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
-typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef float v4 __attribute__((ext_vector_type(4)));
 
 // 16 bytes of the cache as floats
 template <class T>
@@ -225,9 +227,32 @@ __device__ __forceinline__ void attend(const float (&q)[GB][NV][Vec<T>::N], cons
         }
 }
 
+// Scores by the matrix cores: for four heads of whole 32-dim steps whose V rows
+// fill no more than 16 lanes; of hd 96, where a lane holds 24 dims and three
+// heads already leave two waves to a SIMD, also for three.  64 sequences of up
+// to 4201 bf16 rows, 8 KV heads (hd 96 and three heads: 4), against the vector
+// unit (us): 4 heads of 128 98 / 108, of 96 59 / 112, of 64 59 / 66, of 32 37 /
+// 40; 3 heads of 128 57 / 55, of 96 55 / 92, of 64 31 / 28.
+template <class T, int HD, int GB>
+constexpr bool matrix_scores() {
+    return sizeof(T) == 2 && HD % 32 == 0 && HD <= 128 && (GB == 4 || (GB == 3 && HD == 96));
+}
+
+// x of lane i of the quad
+template <int I>
+__device__ __forceinline__ float quad_lane(float x) {
+    return __uint_as_float(
+        __builtin_amdgcn_mov_dpp(__float_as_uint(x), I * 0x55, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float quad_lane(float x, int i) {  // i: a constant where it is used
+    return i == 0 ? quad_lane<0>(x) : i == 1 ? quad_lane<1>(x) : i == 2 ? quad_lane<2>(x)
+                                                                       : quad_lane<3>(x);
+}
+
 // REUSE: another workgroup reads the same keys for other heads.
 template <class T, int HD, int GB, bool REUSE>
 __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(DecodeParams p) {
+    constexpr bool MX = matrix_scores<T, HD, GB>();
     constexpr int LPG = Cfg<T, HD>::LPG, TP = Cfg<T, HD>::TP, N = Vec<T>::N;
     constexpr int NV = HD / LPG / N;
     constexpr int GPW = 64 / LPG;
@@ -271,68 +296,246 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(DecodeParams 
     const int32_t* table = b.table + (size_t)r.seq * b.stride;
     const int slot_mask = (1 << b.ps_shift) - 1;
 
-    float q[GB][NV][N], m[GB], l[GB], o[GB][NV][N];
+    float m[GB], l[GB], o[GB][NV][N];
 #pragma unroll
     for (int i = 0; i < GB; ++i) {
-        // a head group's last workgroup may have fewer heads: it computes one twice
-        const float* src = p.q + ((size_t)ch.row * p.num_heads + g * p.kv_mul +
-                                  min(hb + i, p.kv_mul - 1)) * HD;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int e = 0; e < N; e += 4) {
-                const float4 x = ld4(src + N * (v * LPG + li) + e);
-                q[i][v][e] = x.x * p.scale_log2;
-                q[i][v][e + 1] = x.y * p.scale_log2;
-                q[i][v][e + 2] = x.z * p.scale_log2;
-                q[i][v][e + 3] = x.w * p.scale_log2;
-#pragma unroll
-                for (int f = 0; f < 4; ++f) o[i][v][e + f] = 0.0f;
-            }
+            for (int e = 0; e < N; ++e) o[i][v][e] = 0.0f;
         m[i] = -FLT_MAX;  // finite, so that m - m and score - m need no guard
         l[i] = 0.0f;
     }
-
     bool bad_page = false;
-    int page[TP];
-    const auto key = [&](int tb, int tp) {  // the lane group's key of a tile, clamped to the last
-        return vis.row(min(tb + (tp * kWaves + wave) * GPW + lg, u_end - 1));
+    const size_t to_v = ((size_t)b.kv_heads << b.ps_shift) * HD;
+    const auto load = [](const T* a) {
+        return REUSE ? *reinterpret_cast<const u4*>(a)
+                     : __builtin_nontemporal_load(reinterpret_cast<const u4*>(a));
     };
-    const auto look_up = [&](int tb) {
-#pragma unroll
-        for (int tp = 0; tp < TP; ++tp) page[tp] = table[key(tb, tp) >> b.ps_shift];
+    const auto q_row = [&](int i) {
+        // a head group's last workgroup may have fewer heads: it computes one twice
+        return p.q + ((size_t)ch.row * p.num_heads + g * p.kv_mul + min(hb + i, p.kv_mul - 1)) * HD;
     };
-    if (u_beg < u_end) look_up(u_beg);
-    for (int tb = u_beg; tb < u_end; tb += TILE) {
-        u4 kr[TP][NV], vr[TP][NV];
+    if constexpr (MX) {
+        // A wave has 16 DT keys of a tile.  S^T = K . Q^T by
+        // v_mfma_f32_16x16x32_bf16: A is K as it lies in the page (lane l has
+        // 16-byte pieces of key l % 16); the columns of B are the heads' three
+        // bf16 planes, column 4 p + i plane p of head i.  Lane l ends with the
+        // scores of head l % 4 against keys 4 (l / 16) + r, and the lane groups of
+        // its row of 16 lanes take just these keys' V.  For four heads of 128 that
+        // leaves 14 vector instructions per key of 29.
+        constexpr int DT = TP * GPW / 16, NK = HD / 32, B = 16 / LPG, R = 4 / B;
+        static_assert(TP == DT * R, "a row of 16 lanes takes the V of its four keys");
+        const int row16 = lane >> 4, n = lane & 15, sub = n / LPG;
+        bf8 qf[NK];
+        float scale;
+        {
+            const float* src = q_row(min(n & 3, GB - 1));
+            float x[NK][8], top = 0.0f;
 #pragma unroll
-        for (int tp = 0; tp < TP; ++tp) {
-            const bool ok = paged_page_ok(b, page[tp]);
-            bad_page |= !ok;
-            const T* at = pages + paged_at(b, ok ? page[tp] : 0, 0, g, key(tb, tp) & slot_mask, HD);
-            const size_t to_v = ((size_t)b.kv_heads << b.ps_shift) * HD;
+            for (int i = 0; i < NK; ++i)
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const T* a = at + N * (v * LPG + li);
-                if constexpr (REUSE) {
-                    kr[tp][v] = *reinterpret_cast<const u4*>(a);
-                    vr[tp][v] = *reinterpret_cast<const u4*>(a + to_v);
-                } else {
-                    kr[tp][v] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a));
-                    vr[tp][v] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(a + to_v));
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 y = ld4(src + 8 * (4 * i + row16) + e);
+                    x[i][e] = y.x * p.scale_log2;
+                    x[i][e + 1] = y.y * p.scale_log2;
+                    x[i][e + 2] = y.z * p.scale_log2;
+                    x[i][e + 3] = y.w * p.scale_log2;
+                }
+#pragma unroll
+            for (int i = 0; i < NK; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            // largest magnitude in [2^-10, 2^-9), as for runs of rows
+            int ex = 0;
+            if (top > 0.0f && top < INFINITY) {
+                (void)frexpf(top, &ex);
+                ex += 9;
+            }
+            scale = ldexpf(1.0f, min(max(ex, -126), 127));
+#pragma unroll
+            for (int i = 0; i < NK; ++i) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i][e] = ldexpf(x[i][e], -ex);
+                bf8 w[3];
+                split8(x[i], w);
+                const u4 zero = {0, 0, 0, 0};
+                qf[i] = n < 4 ? w[0] : n < 8 ? w[1] : n < 12 ? w[2]
+                                                             : __builtin_bit_cast(bf8, zero);
+            }
+        }
+        float mh = -FLT_MAX, lh = 0.0f;  // of head lane % 4 and this row of lanes' keys
+        int page[DT];
+        const auto key = [&](int tb, int t, int k) {
+            return vis.row(min(tb + (wave * DT + t) * 16 + k, u_end - 1));
+        };
+        const auto look_up = [&](int tb) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t) page[t] = table[key(tb, t, n) >> b.ps_shift];
+        };
+        if (u_beg < u_end) look_up(u_beg);
+        for (int tb = u_beg; tb < u_end; tb += TILE) {
+            u4 kr[DT][NK], vr[TP][NV];
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const bool ok = paged_page_ok(b, page[t]);
+                bad_page |= !ok;
+                const size_t off =
+                    paged_at(b, ok ? page[t] : 0, 0, g, key(tb, t, n) & slot_mask, HD);
+#pragma unroll
+                for (int i = 0; i < NK; ++i) kr[t][i] = load(pages + off + 8 * (4 * i + row16));
+#pragma unroll
+                for (int s = 0; s < R; ++s) {  // lane k of a row has key k's address
+                    const int k = 4 * row16 + sub * R + s;
+                    const size_t voff = (size_t)(uint32_t)__shfl((int)(off >> 32), k) << 32 |
+                                        (uint32_t)__shfl((int)off, k);
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+                        vr[t * R + s][v] = load(pages + to_v + voff + N * (v * LPG + li));
+                }
+            }
+            if (tb + TILE < u_end) look_up(tb + TILE);
+            v4 sc[DT];
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                v4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < NK; ++i)
+                    s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, kr[t][i]),
+                                                                qf[i], s, 0, 0, 0);
+                // the planes' sum, the same bits in all four lanes of a head
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[r] += __uint_as_float(__builtin_amdgcn_mov_dpp(
+                        __float_as_uint(s[r]), 0x128, 0xF, 0xF, true));  // row_ror:8
+                    s[r] += __uint_as_float(__builtin_amdgcn_mov_dpp(
+                        __float_as_uint(s[r]), 0x124, 0xF, 0xF, true));  // row_ror:4
+                }
+                sc[t] = s * scale;
+            }
+            if (tb + TILE > u_end) {  // uniform: the last keys; what lies behind has no part
+                const int end = u_end - tb - wave * DT * 16;
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        sc[t][r] = 16 * t + 4 * row16 + r < end ? sc[t][r] : -INFINITY;
+#pragma unroll
+                    for (int s = 0; s < R; ++s)
+#pragma unroll
+                        for (int v = 0; v < NV; ++v) {
+                            const bool in = 16 * t + 4 * row16 + sub * R + s < end;
+                            const u4 zero = {0, 0, 0, 0};
+                            vr[t * R + s][v] = in ? vr[t * R + s][v] : zero;
+                        }
+                }
+            }
+            float mx = sc[0][0];
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[t][r]);
+            if (__any(mx > mh + kLazyRescale)) {  // uniform
+                const float mn = fmaxf(mh, mx);
+                const float alpha = fast_exp2(mh - mn);
+                lh *= alpha;
+                mh = mn;
+#pragma unroll
+                for (int i = 0; i < GB; ++i) {
+                    const float a = quad_lane(alpha, i);
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+#pragma unroll
+                        for (int e = 0; e < N; ++e) o[i][v][e] *= a;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    sc[t][r] = fast_exp2(sc[t][r] - mh);
+                    lh += sc[t][r];
+                }
+#pragma unroll
+                for (int s = 0; s < R; ++s) {
+                    float pr = sc[t][s];
+#pragma unroll
+                    for (int k = 1; k < B; ++k) pr = sub == k ? sc[t][k * R + s] : pr;
+                    float pi[GB];
+#pragma unroll
+                    for (int i = 0; i < GB; ++i) pi[i] = quad_lane(pr, i);
+#pragma unroll
+                    for (int v = 0; v < NV; ++v) {
+                        float f[N];
+                        Vec<T>::get(vr[t * R + s][v], f);
+#pragma unroll
+                        for (int i = 0; i < GB; ++i)
+#pragma unroll
+                            for (int e = 0; e < N; ++e)
+                                o[i][v][e] = fmaf(pi[i], f[e], o[i][v][e]);
+                    }
                 }
             }
         }
-        if (tb + TILE < u_end) look_up(tb + TILE);
-        if (tb + TILE <= u_end) {
-            attend<T, HD, LPG, NV, GB, TP, TP>(q, kr, vr, 0, m, l, o);
-        } else {
-            // the last keys: lane groups behind the end sit out, so that what
-            // they loaded is never multiplied
+        bad_page = __any(bad_page);
 #pragma unroll
-            for (int tp = 0; tp < TP; ++tp)
-                if (tb + (tp * kWaves + wave) * GPW + lg < u_end)
-                    attend<T, HD, LPG, NV, GB, 1, TP>(q, kr, vr, tp, m, l, o);
+        for (int i = 0; i < GB; ++i) {
+            m[i] = quad_lane(mh, i);
+            l[i] = sub == 0 ? quad_lane(lh, i) : 0.0f;  // once for a row of lanes
+        }
+    } else {
+        float q[GB][NV][N];
+#pragma unroll
+        for (int i = 0; i < GB; ++i) {
+            const float* src = q_row(i);
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int e = 0; e < N; e += 4) {
+                    const float4 x = ld4(src + N * (v * LPG + li) + e);
+                    q[i][v][e] = x.x * p.scale_log2;
+                    q[i][v][e + 1] = x.y * p.scale_log2;
+                    q[i][v][e + 2] = x.z * p.scale_log2;
+                    q[i][v][e + 3] = x.w * p.scale_log2;
+                }
+        }
+
+        int page[TP];
+        const auto key = [&](int tb, int tp) {  // the lane group's key of a tile, clamped to the last
+            return vis.row(min(tb + (tp * kWaves + wave) * GPW + lg, u_end - 1));
+        };
+        const auto look_up = [&](int tb) {
+#pragma unroll
+            for (int tp = 0; tp < TP; ++tp) page[tp] = table[key(tb, tp) >> b.ps_shift];
+        };
+        if (u_beg < u_end) look_up(u_beg);
+        for (int tb = u_beg; tb < u_end; tb += TILE) {
+            u4 kr[TP][NV], vr[TP][NV];
+#pragma unroll
+            for (int tp = 0; tp < TP; ++tp) {
+                const bool ok = paged_page_ok(b, page[tp]);
+                bad_page |= !ok;
+                const T* at = pages + paged_at(b, ok ? page[tp] : 0, 0, g, key(tb, tp) & slot_mask, HD);
+#pragma unroll
+                for (int v = 0; v < NV; ++v) {
+                    const T* a = at + N * (v * LPG + li);
+                    kr[tp][v] = load(a);
+                    vr[tp][v] = load(a + to_v);
+                }
+            }
+            if (tb + TILE < u_end) look_up(tb + TILE);
+            if (tb + TILE <= u_end) {
+                attend<T, HD, LPG, NV, GB, TP, TP>(q, kr, vr, 0, m, l, o);
+            } else {
+                // the last keys: lane groups behind the end sit out, so that what
+                // they loaded is never multiplied
+#pragma unroll
+                for (int tp = 0; tp < TP; ++tp)
+                    if (tb + (tp * kWaves + wave) * GPW + lg < u_end)
+                        attend<T, HD, LPG, NV, GB, 1, TP>(q, kr, vr, tp, m, l, o);
+            }
         }
     }
 

@@ -100,6 +100,39 @@ def test_large_and_small_values(k_scale, v_scale, q_scale, seqs, dtype):
         check_attention(d.host(d.attend()), b)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(8, 2, 64), (8, 2, 128), (6, 2, 96), (8, 2, 32)])
+@pytest.mark.parametrize("k_scale,v_scale,q_scale", [
+    (1.0, 2.0 ** 70, 1.0), (2.0 ** 80, 1.0, 2.0 ** -80), (2.0 ** -86, 1.0, 2.0 ** 86),
+    (1.0, 2.0 ** -100, 1.0)])
+def test_large_and_small_values_of_single_tokens(heads, kv_heads, hd, k_scale, v_scale, q_scale,
+                                                 dtype):
+    b = Batch(heads, kv_heads, hd, 16, [(m, 1) for m in (1, 70, 0, 130, 2900)], dtype, seed=55,
+              decode=True, q_scale=q_scale)
+    scaled(scaled(b, 0, k_scale), 1, v_scale)
+    with b.upload(torch) as d:
+        check_attention(d.host(d.attend()), b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+def test_nan_and_infinity_stay_in_their_head_and_dimension(hd, dtype):
+    # the last key of a row and one amid a tile; NaN in one row's query
+    b = Batch(8, 2, hd, 16, [(70, 1), (33, 1), (45, 1)], dtype, seed=56, decode=True)
+    want, tol = b.attend64()
+    want, tol = want.reshape(3, 8, hd), tol.reshape(3, 8, hd)
+    b.pool[b.table[0, 4], 1, 0, 5, 7] = math.nan
+    b.pool[b.table[1, 1], 1, 1, 3, 9] = -math.inf
+    b.q[2, 3 * hd + 1] = math.nan
+    with b.upload(torch) as d:
+        got = d.host(d.attend()).reshape(3, 8, hd)
+    assert np.isnan(got[0, :4, 7]).all() and (got[1, 4:, 9] == -math.inf).all()
+    assert np.isnan(got[2, 3]).all()
+    for r, h, c in ((0, slice(0, 4), 7), (1, slice(4, 8), 9), (2, 3, slice(None))):
+        got[r, h, c] = want[r, h, c]
+    assert np.all(np.abs(got - want) <= tol)
+
+
 def test_small_f32_keys():
     b = Batch(8, 2, 64, 16, [(70, 30), (2900, 12)], "f32", seed=45, q_scale=2.0 ** 110)
     scaled(b, 0, 2.0 ** -110)
