@@ -818,11 +818,12 @@ hipError_t launch_k(const Shape& s, PrefillParams p, hipStream_t st) {
     static_assert(tile_bytes<T, HD, KSP>() <= kLds, "the tiles fit a CU");
     const long tiles = tiles_bound(p.b, s.kv_mul, BM);
     // Tiles that leave CUs empty are split into as many chunks as still run side
-    // by side, if that takes four steps or more off the longest (a second launch
-    // to join them costs about 6 us, a step 1.5 to 3).
+    // by side, if that takes two steps or more off the longest (one sequence, hd 64
+    // f32, 128 rows behind 350: 13.2 us, 19.5 with a limit of four steps; bf16, 64
+    // rows alone: 7.4 us, 9.5 with one of one and a half).
     const long ns = s.cus / (tiles * s.num_kv_heads);
     const long steps = (keys_bound(p) + KS - 1) / KS;
-    p.units = ns >= 2 && steps * (ns - 1) >= 4 * ns ? (int)(ns * tiles) : 0;
+    p.units = ns >= 2 && steps * (ns - 1) >= 2 * ns ? (int)(ns * tiles) : 0;
     // (the plan's sums are 32-bit, also of row starts that overlap)
     if (tiles * steps * p.b.n_seqs >= 1L << 30) p.units = 0;
     const long wgs = (tiles + p.units) * s.num_kv_heads;
@@ -839,39 +840,55 @@ hipError_t launch_k(const Shape& s, PrefillParams p, hipStream_t st) {
 
 // Groups of packed rows and key splits of a workgroup, by wgs, the workgroups
 // that 128-row tiles make, and the keys of the longest row.  Four groups share
-// what is staged; key splits put eight waves on a CU that would have four, and
-// shorten the longest workgroup where there are few; a split over workgroups
-// (launch_k) costs a second launch, but needs no merge in LDS.  Measured over
-// 16 to 4096 rows behind 0 and 2000, page 32 (us):
-//   hd 128 bf16, 4 x 1 against 4 x 2: wgs 32, 128 keys 17.5 / 19.7; wgs 128 behind
-//     2000 94 / 79; wgs 512 143 / 121; wgs 1024 423 / 439
-//   hd 128 f32, 4 x 2 against 2 x 2: wgs 32, 128 keys 29.9 / 19.3; wgs 128 behind
-//     2000 177 / 192; 4 x 1 against 4 x 2 at wgs 512 behind 2000 718 / 780
-//   hd 64 bf16, 4 x 2, 2 x 4 and 1 x 8: wgs 18 17.1 / 14.3 / 13.3; wgs 72 behind
-//     2000 44.9 / 56.2 / 64.3; wgs 144 63.8 / 41.9 / 56.4
-//   hd 64 f32, 4 x 2 against 1 x 4: wgs 9 15.6 / 11.1; wgs 36 behind 2000 37.6 / 81.9
-//   hd 256 bf16, 4 x 1 against 2 x 2: wgs 4 28.8 / 22.3; wgs 64 78.4 / 84.6
+// what is staged; key splits put eight waves on a CU that would have four and
+// shorten the longest workgroup, and fewer groups make more workgroups, where
+// there are few, or where those of 128 rows would leave some CUs without one; a
+// split over workgroups (launch_k) costs a second launch, but needs no merge in
+// LDS.  Measured for one sequence, page 32, 256 CUs (us):
+//   hd 128  4 x 1 / 4 x 2 / 2 x 2        bf16                f32
+//     16 rows (wgs 8)                     7.4 / 10.1 / 9.7    9.4 / 12.5 / 12.2
+//     256 rows (wgs 64)                   18.6 / 20.7 / 17.8  23.2 / 25.4 / 22.3
+//     768 rows (wgs 192)                  50.2 / 39.6 / 37.9  96 / 77 / 66
+//     256 rows behind 2000 (wgs 64)       48.7 / 41.8 / 57.7  83 / 71 / 101
+//     2048 rows behind 2000 (wgs 512)     278 / 270 / 312     584 / 586 / 962
+//     4096 rows behind 2000 (wgs 1024)    670 / 707 / 807     1523 / 1533 / 2529
+//     16 rows of 8 heads behind 2000 (2)  32.1 / 25.1 / 24.0  34.8 / 29.2 / 26.7
+//   hd 64   4 x 2 / 2 x 4 / 1 x 8 (f32: 1 x 4)
+//     256 rows (wgs 18)                   12.5 / 10.2 / 9.3   13.5 / 13.5 / 12.5
+//     1024 rows (wgs 72)                  21.0 / 21.1 / 17.2  26.9 / 33.5 / 33.3
+//     2048 rows (wgs 144)                 55.8 / 35.7 / 44.5  89 / 60 / 87
+//     64 rows behind 2000 (wgs 6)         22.4 / 17.1 / 14.7  23.5 / 18.8 / 17.7
+//     256 rows behind 2000 (wgs 18)       20.4 / 17.6 / 18.3  23.4 / 22.6 / 30.6
+//     1024 rows behind 2000 (wgs 72)      37.9 / 49.7 / 56.3  53.7 / 86.8 / 132
+//   hd 256  4 x 1 / 2 x 2
+//     512 rows (wgs 16)                   29.9 / 24.9
+//     1024 rows behind 2000 (wgs 32)      62.7 / 69.7
 template <class T, int HD>
 hipError_t launch_t(const Shape& s, const PrefillParams& p, hipStream_t st) {
     constexpr bool BF = sizeof(T) == 2;
     const long wgs = tiles_bound(p.b, s.kv_mul, 128) * s.num_kv_heads;
-    const long keys = keys_bound(p);
+    const long keys = keys_bound(p), cus = s.cus;
     if constexpr (HD > 128) {
         if constexpr (BF)
-            if (wgs <= s.cus / 8) return launch_k<T, HD, 2, 2>(s, p, st);
-    } else if constexpr (HD > 64) {
-        if constexpr (!BF)
-            if (keys > 32 && wgs <= (keys <= 1024 ? s.cus : s.cus / 8))
+            if (keys > 128 && wgs <= cus / (keys <= 1024 ? 8 : 16))
                 return launch_k<T, HD, 2, 2>(s, p, st);
-        if (wgs >= s.cus * 3 / 8 && wgs < (BF ? 3 : 2) * s.cus)
-            return launch_k<T, HD, 4, 2>(s, p, st);
+    } else if constexpr (HD > 64) {
+        if (keys > 32) {
+            // whole f32 sequences, whose last rows see twice the average: by smaller
+            // workgroups where less than a round of large ones would wait for them
+            const bool uneven = !BF && wgs > cus / 2 && wgs < cus && keys <= 1536 &&
+                                4 * keys * p.b.n_seqs <= 5L * p.b.n_rows;
+            if (wgs <= cus / (keys <= 256 ? 4 : 32) || uneven)
+                return launch_k<T, HD, 2, 2>(s, p, st);
+            if (wgs < 3 * cus) return launch_k<T, HD, 4, 2>(s, p, st);
+        }
     } else if (keys > 64) {
         constexpr bool k8 = tile_bytes<T, HD, 8>() <= kLds;  // or four splits
-        if (wgs <= s.cus / (keys <= 1024 ? 4 : k8 ? 8 : 16))
+        if (wgs <= (keys > 2048 ? cus / (k8 ? 16 : 32) : k8 ? cus * 3 / 8 : cus / 8))
             return launch_k<T, HD, 1, k8 ? 8 : 4>(s, p, st);
-        if (wgs > s.cus / 2 - s.cus / 8 && wgs <= s.cus * 5 / 8)
+        if (wgs <= cus / 8 || (wgs > cus / 2 && wgs <= cus * 3 / 4))
             return launch_k<T, HD, 2, 4>(s, p, st);
-        if (wgs < 3 * s.cus) return launch_k<T, HD, 4, 2>(s, p, st);
+        if (wgs < 3 * cus) return launch_k<T, HD, 4, 2>(s, p, st);
     }
     return launch_k<T, HD, 4, 1>(s, p, st);
 }
