@@ -7,8 +7,9 @@
 //
 // Tiling.  A workgroup has RG groups of 32 packed rows and KSP key splits, a
 // wave for each.  A step stages KSP tiles of 32 keys in LDS, row by row: the
-// next step's rows are on their way from their pages into registers while this
-// one is attended, and the pages of the one after that are being looked up.
+// next steps' rows are on their way from their pages while this one is attended
+// (straight into LDS where they can, else into registers), and the pages of the
+// one after them are being looked up.
 // Keys are numbered without the window's gap (Visible of the workgroup's rows).
 // Per wave and tile, with v_mfma_f32_32x32x16_bf16:
 //   S^T = K . Q^T    A = K rows, B = Q^T (registers): lane (n = l % 32, h = l /
@@ -27,9 +28,10 @@
 // products the three below 2^-25 are left out.  q is first scaled by a power of
 // two per row, so that values of any size stay within bf16's exponents; the
 // scores' scale takes it back.  What cannot be split or must not be multiplied
-// (V from 2^64 on, infinities and NaN among them; with f32 pages also K, and
-// values between 0 and 2^-96, whose remainders run out of exponents) makes the
-// workgroup compute its rows again in plain f32 (attend_again).
+// makes the workgroup compute its rows again in plain f32 (attend_again): an
+// infinity or NaN in a hidden row of V, which leaves one in the sums; where
+// values pass through registers any V from 2^64 on, with f32 pages also K, and
+// values between 0 and 2^-96, whose remainders run out of exponents.
 //
 // What bounds it: the matrix cores for long runs, the softmax and the splitting
 // between the products next.
@@ -83,19 +85,45 @@ constexpr int planes() {
     return sizeof(T) == 2 ? 1 : 3;
 }
 
+// Whether tiles go from the pages straight into LDS: bf16 rows of a power of two
+// of chunks.  64 of them are whole rows of one page then, and land side by side,
+// so the rows cannot be padded: their chunks are exchanged instead, chunk c of row
+// r of a tile lies in slot c ^ swap(r), which the lane that loads it takes into
+// account.  Reads pay an exclusive or each; through registers, with their checks
+// and stores to LDS, the tiles took 95 of the 445 us of 4096 rows, Llama-3-8B
+// shape.
+template <class T, int HD>
+constexpr bool direct() {
+    return sizeof(T) == 2 && HD >= 32 && (HD & (HD - 1)) == 0;
+}
+
+// Distinct for rows that are read together: K takes the same chunk of 16
+// neighbouring rows, V four chunks (4 d ..) of four rows.
+template <int CH>
+__device__ __forceinline__ int swap_of(int row) {
+    const int four = CH >= 16 ? (row & 3) << 2 : CH == 8 ? (row & 2) << 1 : 0;
+    return four | (row >> 2 & 3);
+}
+
 // Bytes of one buffer of K and V tiles in LDS, and what a CU has for them.
 template <class T, int HD, int KSP>
 constexpr int tile_bytes() {
-    return KSP * KT * 16 * planes<T>() * (k_stride(HD / 8) + v_stride(HD / 8));
+    constexpr int ch = HD / 8;
+    return KSP * KT * 16 * planes<T>() *
+           (direct<T, HD>() ? 2 * ch : k_stride(ch) + v_stride(ch));
 }
 constexpr int kLds = 160 * 1024 - 256;
 
 // Two buffers, unless only one lets the CU hold eight waves (where the registers
-// do: q and the output of hd 256 leave room for four).
+// do: q and the output of hd 256 leave room for four).  A third one, where it
+// fits, gives tiles that go straight into LDS two steps to arrive.
 template <class T, int HD, int RG, int KSP>
 constexpr int buffers() {
     constexpr int wgs = RG * KSP == 4 && HD <= 128 ? 2 : 1;
-    return 2 * wgs * tile_bytes<T, HD, KSP>() <= kLds ? 2 : 1;
+    constexpr int most = direct<T, HD>() ? 3 : 2;
+    for (int n = most; n > 1; --n)
+        if (n * wgs * tile_bytes<T, HD, KSP>() <= kLds) return n;
+    return 1;
 }
 
 // Waves of a SIMD that the registers are held to: two, unless the tiles in LDS,
@@ -362,7 +390,8 @@ paged_prefill_kernel(PrefillParams p) {
     constexpr int NQ = HD / 16;            // 16-dim steps of K . Q^T
     constexpr int ND = (HD + 31) / 32;     // 32-dim tiles of O^T
     constexpr bool DPAD = HD % 32 != 0;    // the last of them is half empty
-    constexpr int KST = k_stride(CH), VST = v_stride(CH);
+    constexpr bool DIRECT = direct<T, HD>();
+    constexpr int KST = DIRECT ? CH : k_stride(CH), VST = DIRECT ? CH : v_stride(CH);
     constexpr int MT = KSP == 2 ? (ND + 1) / 2 : ND;  // tiles of O^T that a wave gives away
     // K tiles, then V tiles, NB buffers of NP planes each; at the end the key
     // splits' states
@@ -413,6 +442,7 @@ paged_prefill_kernel(PrefillParams p) {
     // tid + NT, ..  Where the 64 chunks of a wave are whole rows of one page
     // (UNI), the page is looked up and the address formed by the scalar unit.
     constexpr bool UNI = CH >= 4 && (CH & (CH - 1)) == 0;
+    static_assert(!DIRECT || UNI, "a wave's chunks lie side by side");
     const int pos_last = span.pos_last;
     int page[NC];
     u4 kr[NC][NL], vr[NC][NL];
@@ -512,6 +542,63 @@ paged_prefill_kernel(PrefillParams p) {
         }
     };
 
+    // Straight into LDS: buffer loads, whose range makes zeros of the rows behind
+    // the end and of a bad page.  (Inline assembly: the compiler must not make
+    // LDS reads of other tiles wait for them.  M0 has the wave's place in LDS.  The
+    // load must not issue in the cycle after M0 is written, nor in the five after a
+    // vector instruction has written its descriptor.)
+    constexpr int AHEAD = NB - 1;  // steps that loads are issued ahead
+    static_assert(!DIRECT || (NB >= 2 && (EXACT || NC == 1)), "the waits count a step's loads");
+    int src_off[NC];               // where the lane's chunk lies among the wave's
+    unsigned lost_of = 0;          // NC bits per step to come: its pages that are bad
+    if constexpr (DIRECT) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            src_off[i] = ((lane & ~(CH - 1)) +
+                          (lane % CH ^ swap_of<CH>((wave * 64 + i * NT + lane) / CH))) * 16;
+    }
+    const auto load_step = [&](int st, int buf, int ahead) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int e0 = wave * 64 + i * NT;
+            if (!EXACT && e0 >= KS * CH) break;  // uniform
+            const int t = first_row(st, i);
+            const bool ok = paged_page_ok(b, page[i]);
+            if (!ok) lost_of |= 1u << (ahead * NC + i);
+            const int rows = min(64 / CH, max(0, pos_last + 1 - t));
+            const T* at = pages + paged_at(b, ok ? page[i] : 0, 0, g, t & slot_mask, HD);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const uint64_t a = reinterpret_cast<uint64_t>(w ? at + to_v : at);
+                const u4 r = {(uint32_t)__builtin_amdgcn_readfirstlane((int)a),
+                              (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) & 0xFFFF,
+                              (uint32_t)__builtin_amdgcn_readfirstlane(
+                                  ok ? rows * HD * (int)sizeof(T) : 0),
+                              0x00020000u};
+                const unsigned dst = (unsigned)(unsigned long)(
+                    __attribute__((address_space(3))) u4*)((w ? s_v : s_k) + buf * KS * CH + e0);
+                asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(src_off[i]),
+                             "s"(r), "{m0}"(dst) : "memory");
+            }
+        }
+    };
+    // The step's tiles are there, for this wave (later ones may be on their way).
+    const auto arrived = [&](int st, int buf) {
+        if (AHEAD == 2 && st + 1 < st_end)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * NC) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // K of a bad page is NaN, so that the scores of the rows that see it are
+        if (lost_of & ((1u << NC) - 1)) {  // uniform
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (lost_of >> i & 1)
+                    s_k[buf * KS * CH + tid + i * NT] =
+                        u4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+        }
+        lost_of >>= NC;
+    };
+
     // ---- q ----
     // Lane (n, half) holds dims 16 i + 8 half + (0..7) of packed row n, times
     // log2(e) / sqrt(hd) and a power of two, in three planes.
@@ -531,7 +618,10 @@ paged_prefill_kernel(PrefillParams p) {
             for (int e = 0; e < 8; ++e) xq[i][e] = v[e] * p.scale_log2;
         }
         if (any) {
-            fetch(st_beg);
+            if constexpr (DIRECT)
+                load_step(st_beg, 0, 0);
+            else
+                fetch(st_beg);
             if (st_beg + 1 < st_end) look_up(st_beg + 1);
         }
         float top = 0.0f;
@@ -570,13 +660,23 @@ paged_prefill_kernel(PrefillParams p) {
     const auto attend = [&](int buf, int u0) {
         const u4* sk = s_k + (buf * NP * KS + ksp * KT) * KST;
         const u4* sv = s_v + (buf * NP * KS + ksp * KT) * VST;
+        // DIRECT: bytes from there to the lane's chunks 0 (a tile's first byte has
+        // the low bits 0, so the exclusive ors below may follow the sums)
+        const unsigned ka = (unsigned)(n * CH + (half ^ swap_of<CH>(n))) * 16;
+        const int vrow = 4 * half + (lane >> 2 & 3);
+        const unsigned va =
+            (unsigned)(vrow * CH + ((lane >> 3 & 2) + (lane >> 1 & 1) ^ swap_of<CH>(vrow))) * 16 +
+            8 * (lane & 1);
         v16 s = v16{};
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
             bf8 kf[NP];
 #pragma unroll
             for (int k = 0; k < NP; ++k)
-                kf[k] = __builtin_bit_cast(bf8, sk[k * KS * KST + n * KST + 2 * i + half]);
+                kf[k] = __builtin_bit_cast(
+                    bf8, DIRECT ? *reinterpret_cast<const u4*>(reinterpret_cast<const char*>(sk) +
+                                                               (ka ^ 32u * i))
+                                : sk[k * KS * KST + n * KST + 2 * i + half]);
 #pragma unroll
             for (int e = 0; e < NPR; ++e)
                 s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[PA[e]], qb[i][PB[e]], s, 0, 0, 0);
@@ -631,8 +731,12 @@ paged_prefill_kernel(PrefillParams p) {
                     for (int c = 0; c < 2; ++c) {
                         const int row = 16 * ks + 8 * c + 4 * half + ((lane >> 2) & 3);
                         const short* at =
-                            reinterpret_cast<const short*>(sv + k * KS * VST + row * VST) + 32 * d +
-                            dim;
+                            DIRECT ? reinterpret_cast<const short*>(
+                                         reinterpret_cast<const char*>(sv) +
+                                         (16 * ks + 8 * c) * CH * 16 +
+                                         (va ^ (unsigned)(4 * d ^ 2 * c) * 16))
+                                   : reinterpret_cast<const short*>(sv + k * KS * VST + row * VST) +
+                                         32 * d + dim;
                         w[c] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (__attribute__((address_space(3))) s4*)(at));
                     }
@@ -648,24 +752,53 @@ paged_prefill_kernel(PrefillParams p) {
     };
 
     // ---- the steps ----
-    if (st_beg < st_end) {  // uniform
+    // (a wave whose rows are all empty or in front of a tile has nothing to do
+    // there)
+    const auto attend_step = [&](int st, int buf) {
+        const int u0 = st * KS + ksp * KT;
+        if (wave_ok && u0 < vis.count && vis.row(u0) <= wpos_last) attend(buf, u0);
+    };
+    bool outside;
+    if constexpr (DIRECT) {
+        if (AHEAD == 2 && st_beg + 1 < st_end) {
+            load_step(st_beg + 1, 1, 1);
+            if (st_beg + 2 < st_end) look_up(st_beg + 2);
+        }
+        int buf = 0;
         for (int st = st_beg; st < st_end; ++st) {
-            const int u = st * KS, buf = NB == 2 ? st & 1 : 0;
+            arrived(st, buf);
+            __syncthreads();
+            // every wave is done with the buffer of the step before
+            if (st + AHEAD < st_end) {
+                load_step(st + AHEAD, buf == 0 ? NB - 1 : buf - 1, AHEAD - 1);
+                if (st + AHEAD + 1 < st_end) look_up(st + AHEAD + 1);
+            }
+            attend_step(st, buf);
+            buf = buf == NB - 1 ? 0 : buf + 1;
+        }
+        // what must not be multiplied has left an infinity or NaN
+        float x = 0.0f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x = fmaf(o[d][r], 0.0f, x);
+        outside = x != x;
+    } else {
+        for (int st = st_beg; st < st_end; ++st) {
+            const int buf = NB == 2 ? st & 1 : 0;
             stage(st, buf);
             if (st + 1 < st_end) {
                 fetch(st + 1);
                 if (st + 2 < st_end) look_up(st + 2);
             }
             __syncthreads();
-            const int u0 = u + ksp * KT;
-            // a wave whose rows are all empty or in front of the tile has
-            // nothing to do there
-            if (wave_ok && u0 < vis.count && vis.row(u0) <= wpos_last) attend(buf, u0);
+            attend_step(st, buf);
             if (NB == 1) __syncthreads();
         }
+        outside = range.outside();
     }
     l += other_half(l);
-    const bool redo = __syncthreads_or(range.outside());  // (and every wave is done with the tiles)
+    const bool redo = __syncthreads_or(outside);  // (and every wave is done with the tiles)
 
     // ---- key splits ----
     if constexpr (KSP > 1) {
