@@ -979,23 +979,26 @@ hipError_t launch_k(const Shape& s, PrefillParams p, hipStream_t st) {
 // split over workgroups (launch_k) costs a second launch, but needs no merge in
 // LDS.  Measured for one sequence, page 32, 256 CUs (us):
 //   hd 128  4 x 1 / 4 x 2 / 2 x 2        bf16                f32
-//     16 rows (wgs 8)                     7.4 / 10.1 / 9.7    9.4 / 12.5 / 12.2
-//     256 rows (wgs 64)                   18.6 / 20.7 / 17.8  23.2 / 25.4 / 22.3
-//     768 rows (wgs 192)                  50.2 / 39.6 / 37.9  96 / 77 / 66
-//     256 rows behind 2000 (wgs 64)       48.7 / 41.8 / 57.7  83 / 71 / 101
-//     2048 rows behind 2000 (wgs 512)     278 / 270 / 312     584 / 586 / 962
-//     4096 rows behind 2000 (wgs 1024)    670 / 707 / 807     1523 / 1533 / 2529
-//     16 rows of 8 heads behind 2000 (2)  32.1 / 25.1 / 24.0  34.8 / 29.2 / 26.7
+//     16 rows (wgs 8)                     7.4 / 10.3 / 9.4    9.4 / 12.5 / 12.2
+//     256 rows (wgs 64)                   18.4 / 20.6 / 16.8  23.2 / 25.4 / 22.3
+//     512 rows (wgs 128)                  27.4 / 27.0 / 23.8  44.8 / 40.3 / 46.4
+//     768 rows (wgs 192)                  44.3 / 36.2 / 33.8  96 / 77 / 66
+//     64 rows behind 2000 (wgs 16)        25.9 / 26.4 / 24.8  37.0 / 35.8 / 38.5
+//     256 rows behind 2000 (wgs 64)       44.5 / 41.8 / 49.8  83 / 71 / 101
+//     2048 rows behind 2000 (wgs 512)     260 / 249 / 271     584 / 586 / 962
+//     4096 rows behind 2000 (wgs 1024)    629 / 655 / 711     1523 / 1533 / 2529
+//     16 rows of 8 heads behind 2000 (2)  32.1 / 24.9 / 23.7  34.8 / 29.2 / 26.7
 //   hd 64   4 x 2 / 2 x 4 / 1 x 8 (f32: 1 x 4)
-//     256 rows (wgs 18)                   12.5 / 10.2 / 9.3   13.5 / 13.5 / 12.5
-//     1024 rows (wgs 72)                  21.0 / 21.1 / 17.2  26.9 / 33.5 / 33.3
-//     2048 rows (wgs 144)                 55.8 / 35.7 / 44.5  89 / 60 / 87
-//     64 rows behind 2000 (wgs 6)         22.4 / 17.1 / 14.7  23.5 / 18.8 / 17.7
-//     256 rows behind 2000 (wgs 18)       20.4 / 17.6 / 18.3  23.4 / 22.6 / 30.6
-//     1024 rows behind 2000 (wgs 72)      37.9 / 49.7 / 56.3  53.7 / 86.8 / 132
+//     256 rows (wgs 18)                   12.6 / 10.1 / 9.3   13.5 / 13.5 / 12.5
+//     1024 rows (wgs 72)                  20.3 / 19.1 / 17.1  26.9 / 33.5 / 33.3
+//     1536 rows (wgs 108)                 28.3 / 25.1 / 26.6  42.2 / 46.8 / 51.4
+//     2048 rows (wgs 144)                 50.6 / 30.9 / 40.7  89 / 60 / 87
+//     64 rows behind 2000 (wgs 6)         22.3 / 17.4 / 14.9  23.5 / 18.8 / 17.7
+//     256 rows behind 2000 (wgs 18)       20.3 / 17.1 / 17.3  23.4 / 22.6 / 30.6
+//     1024 rows behind 2000 (wgs 72)      35.6 / 42.4 / 48.8  53.7 / 86.8 / 132
 //   hd 256  4 x 1 / 2 x 2
-//     512 rows (wgs 16)                   29.9 / 24.9
-//     1024 rows behind 2000 (wgs 32)      62.7 / 69.7
+//     512 rows (wgs 16)                   29.7 / 24.2
+//     1024 rows behind 2000 (wgs 32)      59.2 / 62.5
 template <class T, int HD>
 hipError_t launch_t(const Shape& s, const PrefillParams& p, hipStream_t st) {
     constexpr bool BF = sizeof(T) == 2;
@@ -1007,11 +1010,13 @@ hipError_t launch_t(const Shape& s, const PrefillParams& p, hipStream_t st) {
                 return launch_k<T, HD, 2, 2>(s, p, st);
     } else if constexpr (HD > 64) {
         if (keys > 32) {
-            // whole f32 sequences, whose last rows see twice the average: by smaller
+            // whole sequences, whose last rows see twice the average: by smaller
             // workgroups where less than a round of large ones would wait for them
-            const bool uneven = !BF && wgs > cus / 2 && wgs < cus && keys <= 1536 &&
+            const bool uneven = wgs > cus / 2 && wgs < cus && keys <= 1536 &&
                                 4 * keys * p.b.n_seqs <= 5L * p.b.n_rows;
-            if (wgs <= cus / (keys <= 256 ? 4 : 32) || uneven)
+            const bool few = BF ? wgs <= cus / (keys <= 512 ? 2 : 16)
+                                : wgs <= cus / (keys <= 256 ? 4 : 32);
+            if (few || uneven)
                 return launch_k<T, HD, 2, 2>(s, p, st);
             if (wgs < 3 * cus) return launch_k<T, HD, 4, 2>(s, p, st);
         }
@@ -1019,7 +1024,7 @@ hipError_t launch_t(const Shape& s, const PrefillParams& p, hipStream_t st) {
         constexpr bool k8 = tile_bytes<T, HD, 8>() <= kLds;  // or four splits
         if (wgs <= (keys > 2048 ? cus / (k8 ? 16 : 32) : k8 ? cus * 3 / 8 : cus / 8))
             return launch_k<T, HD, 1, k8 ? 8 : 4>(s, p, st);
-        if (wgs <= cus / 8 || (wgs > cus / 2 && wgs <= cus * 3 / 4))
+        if (wgs <= cus / 8 || (wgs > cus * (BF ? 3 : 4) / 8 && wgs <= cus * 3 / 4))
             return launch_k<T, HD, 2, 4>(s, p, st);
         if (wgs < 3 * cus) return launch_k<T, HD, 4, 2>(s, p, st);
     }
