@@ -17,8 +17,8 @@
 // ceil(T_r / C) chunks, at most U + n_rows together, which is the grid;
 // workgroups behind the last chunk end at once.  Where C would exceed
 // kLongChunk tiles, more and shorter chunks even out the CUs' loads: up to 4 U, of kChunk
-// tiles at least (64 sequences of up to 4201 rows, Llama-3-8B shape in bf16: 133
-// us with U, 110 us with 4 U; 16 of them 38.1 and 48.8).  A row of one chunk is
+// tiles at least (64 sequences of up to 4201 rows, Llama-3-8B shape in bf16: 118
+// us with U, 99 us with 4 U; 16 of them 35.7 and 38.8).  A row of one chunk is
 // written to out directly.
 //
 // Lanes.  LPG lanes hold one key's head_dim values in 16-byte loads, so a wave
@@ -264,9 +264,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(DecodeParams 
     // Workgroups go to the XCDs round-robin: the nhb that read the same keys for
     // different heads are kXcds apart, so that one L2 serves them all, by plain
     // loads (16 sequences of up to 4201 rows, 8 heads to the KV head at hd 128: f32
-    // 33.6 us side by side, 26.5 apart, 24.7 with plain loads; bf16 25.7, 24.7,
-    // 23.8).  Keys read once keep nontemporal loads (64 sequences, 4 heads: f32 185
-    // us against 202).
+    // 32.2 us side by side, 23.3 apart, 25.1 with nontemporal loads; bf16 22.1,
+    // 18.2, 21.0).  Keys read once keep nontemporal loads (64 sequences, 4 heads:
+    // f32 182 us against 202, bf16 99 against 109).
     const int nhb = (p.kv_mul + GB - 1) / GB;
     const int eight = blockIdx.x / kXcds;
     const int pair = eight / nhb * kXcds + blockIdx.x % kXcds;  // of a chunk and a KV head
