@@ -34,7 +34,10 @@
 // values between 0 and 2^-96, whose remainders run out of exponents.
 //
 // What bounds it: the matrix cores for long runs, the softmax and the splitting
-// between the products next.
+// between the products next.  Measured, Llama-3-8B shape: 4096 rows, bf16 (137
+// GFLOP) 311 us back to back and 392 alone, 442 TFLOP/s in three products each,
+// which is the rate of a large library product; behind 2000 rows 630 us alone (436),
+// f32 1450 to 1550 (180, six products each); 512 rows bf16 23.8 us.
 #include <float.h>
 #include <math.h>
 
@@ -878,7 +881,7 @@ paged_prefill_kernel(PrefillParams p) {
 }
 
 // Joins the chunks of a tile for one KV head: four dims of a packed row per
-// thread.
+// thread.  Bound by its launch and two round trips to memory: 4.2 us.
 template <int HD, int BM, int KS>
 __global__ __launch_bounds__(kThreads) void paged_prefill_join_kernel(PrefillParams p) {
     constexpr int PARTS = (BM * HD / 4 + kThreads - 1) / kThreads;  // workgroups of a tile
