@@ -313,3 +313,46 @@ def test_nothing_but_empty_sequences(decode):
         torch.cuda.synchronize()
         assert np.all(d.host(d.append()) == SENTINEL)
         assert d.pool.isnan().all().item()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hd,heads,kv_heads", [(64, 6, 2), (128, 8, 2), (48, 4, 4)])
+def test_rows_in_front_of_the_first_sequence(hd, heads, kv_heads, dtype):
+    # row_start[0] = 3: rows 0 to 2 belong to no sequence, nor do the last two
+    b = Batch(heads, kv_heads, hd, 16, [(40, 7), (90, 33), (9, 9)], dtype, seed=61, tail=5)
+    want, tol = b.attend64(20, 3)
+    q = np.concatenate([b.q[b.rows:b.rows + 3], b.q[:b.rows], b.q[b.rows + 3:]])
+    with b.upload(torch) as d:
+        d.q.copy_(torch.from_numpy(q))
+        d.row_start += 3
+        torch.cuda.synchronize()
+        got = d.host(d.attend(20, 3))
+        assert np.all(got[:3] == SENTINEL) and np.all(got[b.rows + 3:] == SENTINEL)
+        assert np.all(np.abs(got[3:b.rows + 3] - want[:b.rows]) <= tol[:b.rows])
+        d.out.fill_(SENTINEL)
+        torch.cuda.synchronize()
+        out = d.host(d.append())
+        assert np.all(out[:3] == SENTINEL) and np.all(out[b.rows + 3:] == SENTINEL)
+        assert not np.any(out[3:b.rows + 3] == SENTINEL)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 2), (9000, 1)])
+def test_a_bound_far_above_the_lengths(decode, dtype, window, sinks):
+    seqs = [(m, 1 if decode else r) for m, r in ((5, 5), (0, 2), (130, 40), (17, 1), (64, 64))]
+    b = Batch(8, 2, 128, 16, seqs, dtype, seed=62, decode=decode, stride_extra=2000)
+    b.max_len = 30000
+    with b.upload(torch) as d:
+        check_attention(d.host(d.attend(window, sinks)), b, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_windows_of_rows_in_front_of_the_sequence(dtype):
+    # more rows than positions, with a window: the rows in front are zeros
+    b = Batch(8, 2, 128, 16, [(20, 50), (200, 230), (1, 40)], dtype, seed=63)
+    with b.upload(torch) as d:
+        got = d.host(d.attend(6, 2))
+        for r, _, p in b.positions():
+            assert p >= 0 or np.all(got[r] == 0)
+        check_attention(got, b, 6, 2)
